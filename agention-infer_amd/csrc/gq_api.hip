@@ -7,6 +7,8 @@
 // (src/error.rs:4-42).
 #include <hip/hip_runtime.h>
 
+#include <climits>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -18,6 +20,7 @@
 #include "../../include/gq.h"
 #include "gq_device.h"
 #include "gq_internal.h"
+#include "gq_paged.h"
 
 namespace {
 
@@ -1053,6 +1056,171 @@ int gq_model_prefill(gq_model *m, const int *tokens_host, int n, int pos, float 
     }
   }
   return GQ_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------- many requests over a paged 8-bit cache
+namespace {
+// Arguments are checked before the device is touched, so that a refusal is
+// the same with and without one.
+bool activation_type(int t) { return t == gq::T_F32 || t == gq::T_F16 || t == gq::T_BF16; }
+size_t activation_bytes(int t) { return t == gq::T_F32 ? 4 : 2; }
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_page(int page_size) {
+  if (page_size < 16 || page_size % 16 || page_size > gq::KV8_PAGE_MAX)
+    return fail(GQ_EINVAL, "page_size %d: a multiple of 16 up to %d is needed", page_size, gq::KV8_PAGE_MAX);
+  return GQ_OK;
+}
+
+int check_kv8(const gq_kv8 *c) {
+  if (!c) return fail(GQ_EINVAL, "null cache");
+  if (int rc = check_page(c->page_size)) return rc;
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(GQ_EINVAL, "head_dim %d: 64 or 128 is needed", c->head_dim);
+  if (c->n_kv_heads < 1 || c->n_kv_heads > 65535) return fail(GQ_EINVAL, "%d KV heads", c->n_kv_heads);
+  if (c->n_pages < 1 || (int64_t)c->n_pages * c->page_size > INT_MAX)
+    return fail(GQ_EINVAL, "%d pages of %d tokens: 1 to 2^31 - 1 slots are needed", c->n_pages, c->page_size);
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(GQ_EINVAL, "null cache buffer");
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(GQ_EINVAL, "cache codes must start at a multiple of 16 bytes");
+  return GQ_OK;
+}
+
+int check_type(const char *what, int dtype) {
+  if (!activation_type(dtype)) return fail(GQ_EDTYPE, "%s: unsupported dtype %s", what, type_name(dtype));
+  return GQ_OK;
+}
+
+// Rows of `width` values, `stride` apart, read and written in 16-byte vectors.
+int check_rows(const char *what, const void *p, int64_t stride, int64_t width, int dtype) {
+  if (!p) return fail(GQ_EINVAL, "null %s", what);
+  if (stride < width) return fail(GQ_EINVAL, "%s: rows of %lld values, %lld apart", what, (long long)width, (long long)stride);
+  if (!aligned16(p) || stride * (int64_t)activation_bytes(dtype) % 16)
+    return fail(GQ_EINVAL, "%s: its start and stride must be multiples of 16 bytes", what);
+  return GQ_OK;
+}
+
+int launched(const char *what, hipError_t e) {
+  return e == hipSuccess ? GQ_OK : fail(GQ_EHIP, "%s launch failed: %s", what, hipGetErrorString(e));
+}
+}  // namespace
+
+extern "C" {
+int gq_page_plan(const int *cached_dev, const int *new_dev, int n_requests, int page_size,
+                 const int *free_pages_dev, int n_free, int *tables_dev, int max_pages, int *q_start_dev,
+                 int *ctx_lens_dev, int *positions_dev, int *slots_dev, int max_tokens, int *counts_dev,
+                 void *stream) {
+  if (int rc = check_page(page_size)) return rc;
+  if (n_requests < 0 || n_requests > gq::PAGE_PLAN_MAX_REQUESTS)
+    return fail(GQ_EINVAL, "gq_page_plan: %d requests (at most %d)", n_requests, gq::PAGE_PLAN_MAX_REQUESTS);
+  if (n_free < 0 || max_pages < 0 || max_tokens < 0)
+    return fail(GQ_EINVAL, "gq_page_plan: negative size (n_free %d, max_pages %d, max_tokens %d)", n_free, max_pages,
+                max_tokens);
+  if ((n_requests && (!cached_dev || !new_dev || !ctx_lens_dev)) || (n_requests && max_pages && !tables_dev) ||
+      (n_free && !free_pages_dev) || !q_start_dev || !counts_dev || (max_tokens && (!positions_dev || !slots_dev)))
+    return fail(GQ_EINVAL, "gq_page_plan: null buffer");
+  if (int rc = ensure_init()) return rc;
+  const gq::PagePlanArgs a{cached_dev,    new_dev,   free_pages_dev, tables_dev, q_start_dev, ctx_lens_dev, positions_dev,
+                           slots_dev,     counts_dev, n_requests,    page_size,  max_pages,   n_free,       max_tokens};
+  return launched("page plan", gq::launch_page_plan(a, (hipStream_t)stream));
+}
+
+int gq_rope_freqs(const gq_rope_desc *d, double *inv_freq_host, float *mscale) {
+  if (!d || !inv_freq_host || !mscale) return fail(GQ_EINVAL, "gq_rope_freqs: null argument");
+  if (d->rot_dim < 2 || d->rot_dim % 2) return fail(GQ_EINVAL, "rot_dim %d: an even number is needed", d->rot_dim);
+  if (d->scaling < GQ_ROPE_NONE || d->scaling > GQ_ROPE_LLAMA3) return fail(GQ_EINVAL, "unknown RoPE scaling %d", d->scaling);
+  if (!(d->theta > 1) || !std::isfinite(d->theta) || !(d->attn_factor > 0) || !std::isfinite(d->attn_factor))
+    return fail(GQ_EINVAL, "RoPE theta %g, attn_factor %g: theta > 1 and attn_factor > 0 are needed", d->theta, d->attn_factor);
+  if (d->scaling != GQ_ROPE_NONE && (!(d->factor >= 1) || !std::isfinite(d->factor)))
+    return fail(GQ_EINVAL, "RoPE scaling factor %g: 1 or more is needed", d->factor);
+  if (d->scaling >= GQ_ROPE_YARN && (!(d->orig_ctx > 0) || !std::isfinite(d->orig_ctx)))
+    return fail(GQ_EINVAL, "RoPE orig_ctx %g: the trained context is needed", d->orig_ctx);
+  if (d->scaling == GQ_ROPE_YARN && !(d->beta_slow > 0 && d->beta_fast > d->beta_slow))
+    return fail(GQ_EINVAL, "YaRN betas %g, %g: fast > slow > 0 are needed", d->beta_fast, d->beta_slow);
+  if (d->scaling == GQ_ROPE_LLAMA3 && !(d->low_freq > 0 && d->high_freq > d->low_freq))
+    return fail(GQ_EINVAL, "RoPE low_freq %g, high_freq %g: high > low > 0 are needed", d->low_freq, d->high_freq);
+  const int h = d->rot_dim / 2;
+  for (int i = 0; d->freq_factors && i < h; i++)
+    if (!(d->freq_factors[i] > 0)) return fail(GQ_EINVAL, "RoPE frequency factor %d is %g", i, (double)d->freq_factors[i]);
+  const double pi2 = 6.283185307179586;
+  double lo = 0, hi = 0;
+  if (d->scaling == GQ_ROPE_YARN) {  // the dims of beta_fast and beta_slow turns over the trained context
+    auto dim = [&](double turns) {
+      return d->rot_dim * std::log(d->orig_ctx / (turns * pi2)) / (2 * std::log(d->theta));
+    };
+    lo = std::max(0.0, std::floor(dim(d->beta_fast)));
+    hi = std::min(d->rot_dim - 1.0, std::ceil(dim(d->beta_slow)));
+  }
+  for (int i = 0; i < h; i++) {
+    double f = std::pow(d->theta, -2.0 * i / d->rot_dim);
+    double keep = 1;  // how much of the unscaled frequency stays
+    if (d->scaling == GQ_ROPE_LINEAR) keep = 0;
+    if (d->scaling == GQ_ROPE_YARN) keep = 1 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 1e-3)));
+    if (d->scaling == GQ_ROPE_LLAMA3)
+      keep = std::min(1.0, std::max(0.0, (d->orig_ctx * f / pi2 - d->low_freq) / (d->high_freq - d->low_freq)));
+    if (d->scaling != GQ_ROPE_NONE) f = f * keep + f / d->factor * (1 - keep);
+    inv_freq_host[i] = d->freq_factors ? f / d->freq_factors[i] : f;
+  }
+  *mscale = (float)(d->scaling == GQ_ROPE_YARN ? d->attn_factor * (0.1 * std::log(d->factor) + 1) : d->attn_factor);
+  return GQ_OK;
+}
+
+int gq_rope(int dtype, int layout, int n, int head_dim, int rot_dim, const double *inv_freq_dev, float mscale,
+            const int *pos_dev, const void *q_dev, int64_t q_stride, int n_heads, void *q_out_dev,
+            int64_t q_out_stride, const void *k_dev, int64_t k_stride, int n_kv_heads, void *k_out_dev,
+            int64_t k_out_stride, void *stream) {
+  if (int rc = check_type("gq_rope", dtype)) return rc;
+  if (layout != GQ_ROPE_HALF && layout != GQ_ROPE_INTERLEAVED) return fail(GQ_EINVAL, "unknown RoPE layout %d", layout);
+  if (!k_dev) n_kv_heads = 0, k_stride = k_out_stride = 0, k_out_dev = nullptr;
+  if (n < 0 || n_heads < 1 || n_kv_heads < 0 || n_heads > 65535 || n_kv_heads > 65535 || head_dim < 2 || head_dim > 4096 ||
+      rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim)
+    return fail(GQ_EINVAL, "gq_rope: %d tokens, %d and %d heads of %d (at most 4096), %d of them turned (even)", n, n_heads,
+                n_kv_heads, head_dim, rot_dim);
+  if (n == 0) return GQ_OK;
+  if (!inv_freq_dev || !pos_dev || !q_dev || !q_out_dev || (k_dev && !k_out_dev)) return fail(GQ_EINVAL, "gq_rope: null buffer");
+  const int64_t qw = (int64_t)n_heads * head_dim, kw = (int64_t)n_kv_heads * head_dim;
+  if (q_stride < qw || q_out_stride < qw || k_stride < kw || k_out_stride < kw)
+    return fail(GQ_EINVAL, "gq_rope: a stride is shorter than its row");
+  if ((q_dev == q_out_dev && q_stride != q_out_stride) || (k_dev && k_dev == k_out_dev && k_stride != k_out_stride))
+    return fail(GQ_EINVAL, "gq_rope: in place needs the same stride");
+  if (int rc = ensure_init()) return rc;
+  const gq::RopeArgs a{inv_freq_dev, pos_dev,  q_dev,        k_dev,        q_out_dev, k_out_dev, q_stride,
+                       k_stride,     q_out_stride, k_out_stride, mscale, n, head_dim, rot_dim,
+                       layout == GQ_ROPE_HALF, n_heads, n_kv_heads};
+  return launched("rope", gq::launch_rope(a, dtype, (hipStream_t)stream));
+}
+
+int gq_kv8_append(const gq_kv8 *c, int dtype, const void *k_dev, int64_t k_stride, const void *v_dev,
+                  int64_t v_stride, const int *slots_dev, int n, void *stream) {
+  if (int rc = check_kv8(c)) return rc;
+  if (int rc = check_type("gq_kv8_append", dtype)) return rc;
+  if (n < 0) return fail(GQ_EINVAL, "negative token count %d", n);
+  if (n == 0) return GQ_OK;
+  const int64_t w = (int64_t)c->n_kv_heads * c->head_dim;
+  if (int rc = check_rows("k", k_dev, k_stride, w, dtype)) return rc;
+  if (int rc = check_rows("v", v_dev, v_stride, w, dtype)) return rc;
+  if (!slots_dev) return fail(GQ_EINVAL, "null slots");
+  if (int rc = ensure_init()) return rc;
+  const gq::AppendArgs a{c->k,     c->v,      c->k_scale,    c->v_scale,   k_dev, v_dev, k_stride, v_stride,
+                         slots_dev, n, c->n_kv_heads, c->page_size, c->n_pages * c->page_size};
+  return launched("kv8 append", gq::launch_kv8_append(a, dtype, c->head_dim, (hipStream_t)stream));
+}
+
+int gq_kv8_read(const gq_kv8 *c, const int *slots_dev, int n, int dtype, void *k_out_dev, void *v_out_dev,
+                void *stream) {
+  if (int rc = check_kv8(c)) return rc;
+  if (int rc = check_type("gq_kv8_read", dtype)) return rc;
+  const int64_t w = (int64_t)c->n_kv_heads * c->head_dim;
+  if (n < 0 || n * w / 1024 > INT_MAX) return fail(GQ_EINVAL, "gq_kv8_read: %d tokens in one call", n);
+  if (n == 0 || (!k_out_dev && !v_out_dev)) return GQ_OK;
+  for (const void *p : {k_out_dev, v_out_dev})
+    if (p)
+      if (int rc = check_rows("output", p, w, w, dtype)) return rc;
+  if (!slots_dev) return fail(GQ_EINVAL, "null slots");
+  if (int rc = ensure_init()) return rc;
+  const gq::ReadArgs a{c->k, c->v, c->k_scale, c->v_scale, slots_dev, k_out_dev, v_out_dev, n, c->n_kv_heads, c->head_dim,
+                       c->page_size, c->n_pages * c->page_size};
+  return launched("kv8 read", gq::launch_kv8_read(a, dtype, (hipStream_t)stream));
 }
 
 int gq_sync(void *stream) {

@@ -25,6 +25,7 @@
 
 namespace gq {
 
+enum : int { T_F32 = 0, T_F16 = 1, T_BF16 = 30 };
 enum : int { T_Q8_0 = 8, T_Q4_K = 12, T_Q5_K = 13, T_Q6_K = 14, T_IQ3_XXS = 18 };
 // Kernel-side id (not a ggml type) of Q5_K weights dotted against an input
 // quantized to Q8_K, the route WeightMap::matmul_into takes for Q5_K

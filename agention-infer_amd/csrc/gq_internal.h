@@ -284,4 +284,49 @@ size_t gemm_part_floats(const gq_weight *const *ws, int count, int n, bool quad,
 // rounded up to GEMM_NPAD, zero padding).
 hipError_t launch_x_to_frag(const float *X, int n, int k, uint16_t *xb, hipStream_t st);
 
+// ---- many requests over a paged 8-bit cache (gq_paged.hip) -------------
+struct PagePlanArgs {
+  const int *cached, *fresh;  // [n] tokens in the cache, tokens of this pass
+  const int *free_pages;      // [n_free]
+  int *tables;                // [n][wide]
+  int *q_start;               // [n + 1]
+  int *ctx_lens;              // [n]
+  int *positions, *slots;     // [max_tokens]
+  int *counts;                // tokens, pages taken
+  int n, page, wide, n_free, max_tokens;
+};
+hipError_t launch_page_plan(const PagePlanArgs &a, hipStream_t st);
+
+// Strides in values, between tokens; a head's values are contiguous.
+struct RopeArgs {
+  const double *inv_freq;  // [rot / 2] radians a position
+  const int *pos;          // [n]
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t q_stride, k_stride, q_out_stride, k_out_stride;
+  float mscale;
+  int n, hd, rot, half, nq, nk;
+};
+hipError_t launch_rope(const RopeArgs &a, int dtype, hipStream_t st);
+
+// The cache's fields: codes [pages][heads][page][hd], scales [pages][heads].
+struct AppendArgs {
+  int8_t *kc, *vc;
+  float *ks, *vs;
+  const void *k, *v;
+  int64_t k_stride, v_stride;
+  const int *slots;
+  int n, heads, page, total;  // total: slots of the cache
+};
+hipError_t launch_kv8_append(const AppendArgs &a, int dtype, int hd, hipStream_t st);
+
+struct ReadArgs {
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  const int *slots;
+  void *k_out, *v_out;  // [n][heads][hd]; either may be null
+  int n, heads, hd, page, total;
+};
+hipError_t launch_kv8_read(const ReadArgs &a, int dtype, hipStream_t st);
+
 }  // namespace gq

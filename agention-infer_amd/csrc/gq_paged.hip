@@ -1,0 +1,406 @@
+// gq_paged.hip -- what a pass over many requests does around its attention:
+// page tables and slots from the requests' lengths, rotary positions, and the
+// new k and v rows into pages of 8-bit codes (and back).
+//
+// The cache.  Pages of `page_size` tokens; page p of KV head h holds its rows
+// at codes[p][h][0 .. page_size)[head_dim], so that the rows one head's
+// attention reads are one run of page_size * head_dim bytes; one f32 scale
+// for each (page, head), of k and of v: value = code * scale.
+#include "gq_device.h"
+#include "gq_internal.h"
+#include "gq_paged.h"
+
+namespace gq {
+
+// ------------------------------------------------------------- page plan
+// Request i has cached[i] tokens in the cache and new[i] to come.  With c, n
+// their values, P tokens a page and tables of M pages,
+//   before_i = min(ceil(c / P), M), need_i = min(ceil((c + n) / P), M) - before_i,
+//   tok0_i = sum_{j < i} n_j, pg0_i = sum_{j < i} need_j;
+// table entry before_i + k (k < need_i) is free[pg0_i + k] (-1 past n_free), and
+// token t of the pass, tok0_i <= t < tok0_{i+1}, has position c + t - tok0_i and
+// slot table[position / P] * P + position % P.
+//
+// Launch bound: a few KB in, 8 bytes a token out.  Every block makes both
+// prefix sums in its own LDS (the lengths come from the L2) and then takes its
+// share of the tokens and of the new pages, finding their request by bisection:
+// one launch, and no block waits for another.  The entry that a token reads is
+// either older than this call or recomputed from the free list, so it does not
+// matter which block writes it when.
+constexpr int PLAN_THREADS = 256;
+__global__ __launch_bounds__(PLAN_THREADS) void k_page_plan(PagePlanArgs a) {
+  extern __shared__ int plan_lds[];
+  int *tok0 = plan_lds, *pg0 = plan_lds + a.n + 1;
+  __shared__ int wsum[2][PLAN_THREADS / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.n + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int i0 = min(tid * per, a.n), i1 = min(i0 + per, a.n);
+  auto before = [&](int r) { return pages_of(not_negative(a.cached[r]), a.page, a.wide); };
+  auto need = [&](int r) {
+    const int c = not_negative(a.cached[r]), all = sat_add(c, not_negative(a.fresh[r]));
+    return pages_of(all, a.page, a.wide) - pages_of(c, a.page, a.wide);
+  };
+  int st = 0, sp = 0;
+  for (int r = i0; r < i1; r++) {
+    st = sat_add(st, not_negative(a.fresh[r]));
+    sp = sat_add(sp, need(r));
+  }
+  int xt = st, xp = sp;  // inclusive scan over the wave
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int ot = __shfl_up(xt, off, 64), op = __shfl_up(xp, off, 64);
+    if (lane >= off) {
+      xt = sat_add(xt, ot);
+      xp = sat_add(xp, op);
+    }
+  }
+  if (lane == 63) {
+    wsum[0][wave] = xt;
+    wsum[1][wave] = xp;
+  }
+  // (exclusive: what the lanes below add up to)
+  int et = __shfl_up(xt, 1, 64), ep = __shfl_up(xp, 1, 64);
+  if (lane == 0) et = ep = 0;
+  __syncthreads();
+  for (int w = 0; w < wave; w++) {
+    et = sat_add(et, wsum[0][w]);
+    ep = sat_add(ep, wsum[1][w]);
+  }
+  for (int r = i0; r < i1; r++) {
+    tok0[r] = et;
+    pg0[r] = ep;
+    et = sat_add(et, not_negative(a.fresh[r]));
+    ep = sat_add(ep, need(r));
+  }
+  if (tid == PLAN_THREADS - 1) {  // (its range ends at n)
+    tok0[a.n] = et;
+    pg0[a.n] = ep;
+  }
+  __syncthreads();
+  const int tokens = tok0[a.n], pages = pg0[a.n];
+  if (blockIdx.x == 0) {
+    for (int r = tid; r <= a.n; r += PLAN_THREADS) a.q_start[r] = tok0[r];
+    for (int r = tid; r < a.n; r += PLAN_THREADS)
+      a.ctx_lens[r] = sat_add(not_negative(a.cached[r]), not_negative(a.fresh[r]));
+    if (tid == 0) {
+      a.counts[0] = tokens;
+      a.counts[1] = pages;
+    }
+  }
+  const int64_t step = (int64_t)gridDim.x * PLAN_THREADS, me = (int64_t)blockIdx.x * PLAN_THREADS + tid;
+  for (int64_t g = me; g < pages; g += step) {
+    const int r = owner_of(pg0, a.n, (int)g);
+    a.tables[(int64_t)r * a.wide + before(r) + ((int)g - pg0[r])] = g < a.n_free ? a.free_pages[g] : -1;
+  }
+  for (int64_t t = me; t < a.max_tokens; t += step) {
+    int pos = 0, slot = -1;  // behind the last request: no slot
+    if (t < tokens) {
+      const int r = owner_of(tok0, a.n, (int)t);
+      pos = sat_add(not_negative(a.cached[r]), (int)t - tok0[r]);
+      const int j = pos / a.page, b = before(r);
+      if (j < a.wide) {
+        int id = -1;
+        if (j < b)
+          id = a.tables[(int64_t)r * a.wide + j];
+        else if (const int g = sat_add(pg0[r], j - b); g < a.n_free)
+          id = a.free_pages[g];
+        slot = slot_of(id, a.page, pos % a.page);
+      }
+    }
+    a.positions[t] = pos;
+    a.slots[t] = slot;
+  }
+}
+
+hipError_t launch_page_plan(const PagePlanArgs &a, hipStream_t st) {
+  const int work = a.max_tokens > a.n ? a.max_tokens : a.n;
+  int blocks = (work + PLAN_THREADS - 1) / PLAN_THREADS;
+  blocks = blocks < 1 ? 1 : blocks > 512 ? 512 : blocks;
+  hipLaunchKernelGGL(k_page_plan, dim3(blocks), dim3(PLAN_THREADS), 2 * (size_t)(a.n + 1) * sizeof(int), st, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- types
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return (float)v; }
+template <>
+__device__ __forceinline__ float to_f32<__bf16>(__bf16 v) { return (float)v; }
+
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+// -------------------------------------------------------- rotary positions
+// Pair i of the first `rot` dims of a head (dims i, i + rot / 2 in the half
+// layout, 2 i, 2 i + 1 in the interleaved one) at position p:
+//   a = p * f_i, (y0, y1) = m (x0 cos a - x1 sin a, x0 sin a + x1 cos a).
+// The angle is a 64-bit product reduced to a fraction of a turn in 64 bits
+// (f32 would be off by 0.06 rad at position 10^6); sine and cosine of that
+// fraction are taken in f32.
+//
+// Bound by reading and writing q and k once.  A block is one token: its
+// rot / 2 sines and cosines are made once, in LDS, for all its heads.  A unit
+// is two 16-byte vectors of a half-layout head, or one of an interleaved one;
+// a unit's thread alone reads and writes it, so in place is fine.
+constexpr int ROPE_THREADS = 256;
+template <class T, int VE, bool HALF>
+__global__ __launch_bounds__(ROPE_THREADS) void k_rope(RopeArgs a) {
+  extern __shared__ float2 rope_cs[];  // [rot / 2] m cos, m sin
+  const int t = blockIdx.x, h2 = a.rot / 2;
+  const double pos = (double)a.pos[t];
+  for (int i = threadIdx.x; i < h2; i += ROPE_THREADS) {
+    const double turns = pos * a.inv_freq[i] * 0.15915494309189535;
+    const float x = (float)(2.0 * (turns - rint(turns)));  // half turns in [-1, 1]
+    float s, c;
+    sincospif(x, &s, &c);
+    rope_cs[i] = make_float2(a.mscale * c, a.mscale * s);
+  }
+  __syncthreads();
+  // units of a head: rotated ones, then the ones passed through (VE values)
+  const int ru = HALF ? h2 / VE : a.rot / (VE == 1 ? 2 : VE);
+  const int pu = (a.hd - a.rot) / VE, hu = ru + pu;
+  const int heads = a.nq + a.nk;
+  for (int u = threadIdx.x; u < heads * hu; u += ROPE_THREADS) {
+    const int h = u / hu, w = u % hu;
+    const bool isq = h < a.nq;
+    const T *src = isq ? (const T *)a.q + t * a.q_stride + (int64_t)h * a.hd
+                       : (const T *)a.k + t * a.k_stride + (int64_t)(h - a.nq) * a.hd;
+    T *dst = isq ? (T *)a.q_out + t * a.q_out_stride + (int64_t)h * a.hd
+                 : (T *)a.k_out + t * a.k_out_stride + (int64_t)(h - a.nq) * a.hd;
+    typedef Vec<T, VE> V;
+    if (w >= ru) {
+      const int d = a.rot + (w - ru) * VE;
+      if (src != dst) *(V *)(dst + d) = *(const V *)(src + d);
+    } else if constexpr (HALF || VE == 1) {
+      const int i = w * VE, d0 = HALF ? i : 2 * i, d1 = HALF ? i + h2 : 2 * i + 1;
+      V x0 = *(const V *)(src + d0), x1 = *(const V *)(src + d1);
+#pragma unroll
+      for (int e = 0; e < VE; e++) {
+        const float2 cs = rope_cs[i + e];
+        const float p = to_f32(x0.v[e]), q = to_f32(x1.v[e]);
+        x0.v[e] = (T)fmaf(p, cs.x, -(q * cs.y));
+        x1.v[e] = (T)fmaf(p, cs.y, q * cs.x);
+      }
+      *(V *)(dst + d0) = x0;
+      *(V *)(dst + d1) = x1;
+    } else {
+      V x = *(const V *)(src + w * VE);
+#pragma unroll
+      for (int e = 0; e < VE; e += 2) {
+        const float2 cs = rope_cs[(w * VE + e) / 2];
+        const float p = to_f32(x.v[e]), q = to_f32(x.v[e + 1]);
+        x.v[e] = (T)fmaf(p, cs.x, -(q * cs.y));
+        x.v[e + 1] = (T)fmaf(p, cs.y, q * cs.x);
+      }
+      *(V *)(dst + w * VE) = x;
+    }
+  }
+}
+
+template <class T>
+static void rope_launch(const RopeArgs &a, hipStream_t st) {
+  constexpr int VE = 16 / sizeof(T);
+  const dim3 g(a.n), b(ROPE_THREADS);
+  const size_t lds = (size_t)(a.rot / 2) * sizeof(float2);
+  const int64_t e = VE - 1;
+  auto al = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
+  // 16-byte vectors where every head's rotated and passed parts are whole
+  // ones; else value by value.
+  const bool vec = al(a.q) && al(a.q_out) && al(a.k) && al(a.k_out) &&
+                   !((a.q_stride | a.q_out_stride | a.k_stride | a.k_out_stride) & e) && a.hd % VE == 0 &&
+                   (a.half ? a.rot / 2 : a.rot) % VE == 0;
+  if (vec && a.half)
+    hipLaunchKernelGGL((k_rope<T, VE, true>), g, b, lds, st, a);
+  else if (vec)
+    hipLaunchKernelGGL((k_rope<T, VE, false>), g, b, lds, st, a);
+  else if (a.half)
+    hipLaunchKernelGGL((k_rope<T, 1, true>), g, b, lds, st, a);
+  else
+    hipLaunchKernelGGL((k_rope<T, 1, false>), g, b, lds, st, a);
+}
+
+hipError_t launch_rope(const RopeArgs &a, int dtype, hipStream_t st) {
+  if (dtype == T_F32)
+    rope_launch<float>(a, st);
+  else if (dtype == T_F16)
+    rope_launch<_Float16>(a, st);
+  else
+    rope_launch<__bf16>(a, st);
+  return hipGetLastError();
+}
+
+// ----------------------------------------------------------- cache append
+// The new rows x of one page and head, at offsets [o, o + r), with s the
+// scale there (0 where o = 0: the rows start the page anew):
+//   s' = max(s, max|x| / 127, 2^-60);  earlier rows (offsets < o), if s' > s:
+//   c' = rint(c s / s');  new rows: c = rint(x / s'); ties to even, quotients
+// exact.  A value that is not finite makes s' NaN, and with it what the page
+// holds for that head, until rows start it anew.
+//
+// Bound by reading the rows once (twice from the L2) and writing the codes.
+// A wave takes one run: the tokens t, t + 1, ... whose slots follow each
+// other within a page.  Whether a token begins one shows from its slot and
+// the one before it.
+constexpr int APPEND_THREADS = 64;
+
+// rint(x / s) for finite x, |x| <= 127.5 s, rs = 1 / s (s >= 2^-60): the
+// first guess is off by less than one; the rest of the division, x - c s,
+// is exact in one fma and decides (the tie goes to the even code).
+__device__ __forceinline__ float code_of(float x, float s, float rs) {
+  const float c = rintf(x * rs), rest = fmaf(-c, s, x), h = 0.5f * s;
+  const float up = rest < 0.f ? -1.f : 1.f, far = fabsf(rest);
+  const bool odd = ((int)c & 1) != 0;
+  return far > h || (far == h && odd) ? c + up : c;
+}
+
+template <class T, int HD>
+__global__ __launch_bounds__(APPEND_THREADS) void k_kv8_append(AppendArgs a) {
+  constexpr int VE = 16 / sizeof(T), LPR = HD / VE, RPI = 64 / LPR;  // lanes a row, rows an iteration
+  const int t0 = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+  const bool isv = blockIdx.z;
+  const int slot = a.slots[t0];
+  if (slot < 0 || slot >= a.total) return;
+  const int page = slot / a.page, off = slot % a.page;
+  if (off && t0 && a.slots[t0 - 1] == slot - 1) return;  // inside a run
+  // the run's length: whole groups of 64 followers, then the first that is none
+  int len = 1;
+  const int most = min(a.page - off, a.n - t0);
+  while (len < most) {
+    const int i = len + lane;
+    const unsigned long long no = __ballot(i >= most || a.slots[t0 + i] != slot + i);
+    if (no) {
+      len += __ffsll(no) - 1;
+      break;
+    }
+    len += 64;
+  }
+  const int64_t stride = isv ? a.v_stride : a.k_stride;
+  const T *src = (const T *)(isv ? a.v : a.k) + t0 * stride + (int64_t)h * HD;
+  int8_t *codes = (isv ? a.vc : a.kc) + ((int64_t)page * a.heads + h) * a.page * HD;
+  float *scale = (isv ? a.vs : a.ks) + (int64_t)page * a.heads + h;
+  const int row = lane / LPR, d = (lane % LPR) * VE;
+  typedef Vec<T, VE> V;
+  float top = 0.f;
+  bool bad = false;
+  for (int r = row; r < len; r += RPI) {
+    const V x = *(const V *)(src + r * stride + d);
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+      const float f = fabsf(to_f32(x.v[e]));
+      bad |= !(f <= 3.4028234663852886e38f);
+      top = fmaxf(top, f);
+    }
+  }
+  top = wave_max(top);
+  bad = __any(bad);
+  const float old = off ? *scale : 0.f;
+  // (a NaN held before stays: fmaxf would drop it)
+  const float now = bad || old != old ? __builtin_nanf("") : fmaxf(fmaxf(old, top / 127.0f), KV8_MIN_SCALE);
+  if (now > old && old > 0.f) {
+    const double s0 = old, s1 = now;
+    for (int i = 4 * lane; i < off * HD; i += 256) {
+      const uint32_t w = *(const uint32_t *)(codes + i);
+      uint32_t y = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int c = (int8_t)(w >> (8 * e));
+        y |= ((uint32_t)(int)rint((double)c * s0 / s1) & 0xffu) << (8 * e);
+      }
+      *(uint32_t *)(codes + i) = y;
+    }
+  }
+  const float rs = 1.0f / now;
+  for (int r = row; r < len; r += RPI) {
+    const V x = *(const V *)(src + r * stride + d);
+    uint32_t w[VE / 4];
+#pragma unroll
+    for (int k = 0; k < VE / 4; k++) {
+      w[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        w[k] |= ((uint32_t)(now == now ? (int)code_of(to_f32(x.v[4 * k + e]), now, rs) : 0) & 0xffu) << (8 * e);
+    }
+    int8_t *p = codes + (off + r) * HD + d;
+    if constexpr (VE == 8)
+      *(uint2 *)p = make_uint2(w[0], w[1]);
+    else
+      *(uint32_t *)p = w[0];
+  }
+  if (lane == 0) *scale = now;
+}
+
+template <class T>
+static void append_launch(const AppendArgs &a, int hd, hipStream_t st) {
+  const dim3 g(a.n, a.heads, 2), b(APPEND_THREADS);
+  if (hd == 64)
+    hipLaunchKernelGGL((k_kv8_append<T, 64>), g, b, 0, st, a);
+  else
+    hipLaunchKernelGGL((k_kv8_append<T, 128>), g, b, 0, st, a);
+}
+
+hipError_t launch_kv8_append(const AppendArgs &a, int dtype, int hd, hipStream_t st) {
+  if (dtype == T_F32)
+    append_launch<float>(a, hd, st);
+  else if (dtype == T_F16)
+    append_launch<_Float16>(a, hd, st);
+  else
+    append_launch<__bf16>(a, hd, st);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------- cache read
+// out[t][h][d] = codes[slot_t][h][d] * scale, zeros where there is no slot.
+// Bound by its writes.  A thread makes 16 bytes of output; the grid's second
+// axis is k / v.
+constexpr int READ_THREADS = 256;
+template <class T>
+__global__ __launch_bounds__(READ_THREADS) void k_kv8_read(ReadArgs a) {
+  constexpr int VE = 16 / sizeof(T);
+  const int per = a.heads * a.hd / VE;  // vectors of a token
+  const int64_t g = (int64_t)blockIdx.x * READ_THREADS + threadIdx.x;
+  const int64_t t = g / per;
+  if (t >= a.n) return;
+  const bool isv = a.k_out == nullptr || blockIdx.y == 1;
+  const int c = (int)(g % per) * VE, h = c / a.hd, d = c % a.hd;
+  const int slot = a.slots[t];
+  typedef Vec<T, VE> V;
+  V y;
+  if (slot < 0 || slot >= a.total) {
+#pragma unroll
+    for (int e = 0; e < VE; e++) y.v[e] = (T)0.f;
+  } else {
+    const int64_t ph = (int64_t)(slot / a.page) * a.heads + h;
+    const int8_t *src = (isv ? a.vc : a.kc) + (ph * a.page + slot % a.page) * a.hd + d;
+    const float s = (isv ? a.vs : a.ks)[ph];
+    uint32_t w[VE / 4];
+    if constexpr (VE == 8) {
+      const uint2 u = *(const uint2 *)src;
+      w[0] = u.x;
+      w[1] = u.y;
+    } else {
+      w[0] = *(const uint32_t *)src;
+    }
+#pragma unroll
+    for (int e = 0; e < VE; e++) y.v[e] = (T)((float)(int8_t)(w[e / 4] >> (8 * (e & 3))) * s);
+  }
+  *(V *)((T *)(isv ? a.v_out : a.k_out) + t * a.heads * a.hd + c) = y;
+}
+
+hipError_t launch_kv8_read(const ReadArgs &a, int dtype, hipStream_t st) {
+  const int64_t per = (int64_t)a.heads * a.hd * (dtype == T_F32 ? 4 : 2) / 16;
+  const dim3 g((unsigned)((a.n * per + READ_THREADS - 1) / READ_THREADS), a.k_out && a.v_out ? 2 : 1), b(READ_THREADS);
+  if (dtype == T_F32)
+    hipLaunchKernelGGL(k_kv8_read<float>, g, b, 0, st, a);
+  else if (dtype == T_F16)
+    hipLaunchKernelGGL(k_kv8_read<_Float16>, g, b, 0, st, a);
+  else
+    hipLaunchKernelGGL(k_kv8_read<__bf16>, g, b, 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace gq

@@ -15,6 +15,7 @@ CPU fallback: if libgq.so is missing or no gfx950 is present, calls raise.
 Device buffers are torch tensors on `cuda` (PyTorch is plumbing here: it
 owns device memory and streams; all compute runs in libgq.so).
 """
+import collections
 import ctypes
 import os
 
@@ -28,10 +29,11 @@ GQ_GEMM_INT8 = 1
 
 # GgmlType ids (src/types.rs:9-46)
 Q8_0, Q4_K, Q5_K, Q6_K, IQ3_XXS = 8, 12, 13, 14, 18
+F32, F16, BF16 = 0, 1, 30
 GPU_DEQUANT_DTYPES = (Q8_0, Q4_K, Q5_K, Q6_K)  # src/ops/mod.rs:27-28
 
 # Every entry point declared in include/gq.h, with its ctypes signature.
-_P, _I, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_P, _I, _SZ, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_int64
 SIGNATURES = {
     "gq_init": (_I, [_I]),
     "gq_backend_name": (ctypes.c_char_p, []),
@@ -63,6 +65,11 @@ SIGNATURES = {
     "gq_model_generate": (_I, [_P, _I, _I, _I, _P, _P]),
     "gq_model_prefill": (_I, [_P, _P, _I, _I, _P, ctypes.POINTER(_I), _P]),
     "gq_moe_ffn": (_I, [_P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "gq_page_plan": (_I, [_P, _P, _I, _I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _P, _P]),
+    "gq_rope_freqs": (_I, [_P, _P, ctypes.POINTER(ctypes.c_float)]),
+    "gq_rope": (_I, [_I, _I, _I, _I, _I, _P, ctypes.c_float, _P, _P, _L, _I, _P, _L, _P, _L, _I, _P, _L, _P]),
+    "gq_kv8_append": (_I, [_P, _I, _P, _L, _P, _L, _P, _I, _P]),
+    "gq_kv8_read": (_I, [_P, _P, _I, _I, _P, _P, _P]),
     "gq_moe_ffn_noalloc": (_I, [_P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
 }
 
@@ -238,6 +245,116 @@ class GpuWeightHandle:
         return Y_dev
 
 
+# ---- many requests over a paged 8-bit cache
+PagePlan = collections.namedtuple("PagePlan", "q_start ctx_lens positions slots counts")
+PagePlan.__doc__ = "What HipBackend.page_plan gives (int32 device tensors; see gq_page_plan in gq.h)."
+Kv8Cache = collections.namedtuple("Kv8Cache", "k v k_scale v_scale")
+Kv8Cache.__doc__ = """Buffers of a paged 8-bit cache: codes int8 [n_pages][n_kv_heads][page_size][head_dim], scales
+float32 [n_pages][n_kv_heads]; made by kv8_cache, or any four tensors of these shapes."""
+
+
+def kv8_cache(n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
+    """A cache of n_pages empty pages (pages need no initialisation)."""
+    import torch
+    code = [torch.empty((n_pages, n_kv_heads, page_size, head_dim), dtype=torch.int8, device=device) for _ in "kv"]
+    scale = [torch.empty((n_pages, n_kv_heads), dtype=torch.float32, device=device) for _ in "kv"]
+    return Kv8Cache(*code, *scale)
+
+
+class _Kv8(ctypes.Structure):
+    _fields_ = [(n, _I) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim")] + \
+        [(n, _P) for n in ("k", "v", "k_scale", "v_scale")]
+
+
+class _RopeDesc(ctypes.Structure):
+    _fields_ = [("rot_dim", _I), ("scaling", _I)] + \
+        [(n, ctypes.c_double) for n in ("theta", "factor", "orig_ctx", "beta_fast", "beta_slow", "low_freq",
+                                        "high_freq", "attn_factor")] + [("freq_factors", _P)]
+
+
+_ROPE_SCALING = {"none": 0, "linear": 1, "yarn": 2, "llama3": 3}
+_ROPE_LAYOUT = {"half": 0, "interleaved": 1}
+_ACT = None
+
+
+def rope_freqs(rot_dim, theta=10000.0, scaling="none", factor=1.0, orig_ctx=0, beta_fast=32.0, beta_slow=1.0,
+               low_freq=1.0, high_freq=4.0, attn_factor=1.0, freq_factors=None):
+    """(inv_freq float64[rot_dim / 2], mscale) for HipBackend.rope; scaling:
+    "none", "linear", "yarn" or "llama3" (gq_rope_freqs in gq.h)."""
+    if scaling not in _ROPE_SCALING:
+        raise ValueError(f"RoPE scaling {scaling!r}: one of {sorted(_ROPE_SCALING)} is needed")
+    ff = None
+    if freq_factors is not None:
+        ff = np.ascontiguousarray(freq_factors, np.float32)
+        if ff.shape != (rot_dim // 2,):
+            raise ValueError(f"freq_factors must have rot_dim / 2 = {rot_dim // 2} values")
+    out, m = np.zeros(max(0, rot_dim // 2), np.float64), ctypes.c_float()
+    d = _RopeDesc(rot_dim, _ROPE_SCALING[scaling], theta, factor, orig_ctx, beta_fast, beta_slow, low_freq, high_freq,
+                  attn_factor, ff.ctypes.data if ff is not None else None)
+    _check(lib().gq_rope_freqs(ctypes.byref(d), _ptr(out), ctypes.byref(m)))
+    return out, m.value
+
+
+def _act(t):
+    """GGML type id of an activation tensor's dtype; raises GqError like the library."""
+    global _ACT
+    if _ACT is None:
+        import torch
+        _ACT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    got = _ACT.get(t.dtype)
+    if got is None:
+        raise GqError(-2, f"unsupported dtype {t.dtype}: float32, float16 or bfloat16 is needed")
+    return got
+
+
+def _on_gpu(name, t, dtype, device, shape=None):
+    """A contiguous device tensor of this type (and shape); its pointer."""
+    if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or \
+            (shape is not None and tuple(t.shape) != shape):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor" + (f" of shape {shape}" if shape is not None else "")
+                         + f" on cuda:{device}: got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(name, t, like, heads=None, dim=None):
+    """Activations [n][heads][dim] whose heads and values are contiguous; (pointer, stride between tokens)."""
+    if t.ndim != 3 or (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
+        raise ValueError(f"{name} must be [n][{heads or 'heads'}][{dim or 'head_dim'}]: got {tuple(t.shape)}")
+    if t.dtype != like.dtype or t.get_device() != like.get_device():
+        raise ValueError(f"{name} must be {like.dtype} on {like.device}: got {t.dtype} on {t.device}")
+    n, h, d = t.shape
+    st = t.stride()
+    if st[2] != 1 or (st[1] != d and h > 1) or (n > 1 and st[0] < h * d):
+        raise ValueError(f"{name}: heads and values must be contiguous, rows must not overlap (strides {st})")
+    return t.data_ptr(), st[0] if n > 1 else h * d
+
+
+def _device():
+    import torch
+    return torch.cuda.current_device()
+
+
+def _cache(cache, device):
+    import torch
+    k, v, ks, vs = cache
+    if k.ndim != 4:
+        raise ValueError(f"cache codes must be [n_pages][n_kv_heads][page_size][head_dim]: got {tuple(k.shape)}")
+    n, h, p, d = shape = tuple(k.shape)
+    return _Kv8(n, p, h, d, _on_gpu("cache k", k, torch.int8, device), _on_gpu("cache v", v, torch.int8, device, shape),
+                _on_gpu("cache k_scale", ks, torch.float32, device, (n, h)),
+                _on_gpu("cache v_scale", vs, torch.float32, device, (n, h)))
+
+
+def _kept(stream, *made):
+    """Tensors made here for a call on `stream` stay allocated until that stream is done with them."""
+    if stream is not None:
+        import torch
+        s = torch.cuda.ExternalStream(stream)
+        for t in made:
+            if t is not None:
+                t.record_stream(s)
+
+
 class HipBackend:
     """The HIP arm of AnyBackend (src/ops/backend_select.rs:25-56)."""
 
@@ -332,6 +449,91 @@ class HipBackend:
         _check(fn(gate._h, up._h, down._h, n_experts, _ptr(logits_dev), T, top_k,
                   _ptr(x_dev), _ptr(out_dev), _ptr(ids), _ptr(w), _stream(stream)))
         return (out_dev, ids, w) if want_routing else out_dev
+
+    # ---- many requests over a paged 8-bit cache (device tensors in and out,
+    # asynchronous on `stream`, the current stream by default)
+    def page_plan(self, cached, new, page_size, free_pages, tables, max_tokens, stream=None):
+        """gq_page_plan: int32 cached[n], new[n], free_pages[m] and
+        tables[n][max_pages] (new pages are written into it) -> PagePlan."""
+        import torch
+        dev, i32 = _device(), torch.int32
+        n = cached.shape[0]
+        c, m = _on_gpu("cached", cached, i32, dev, (n,)), _on_gpu("new", new, i32, dev, (n,))
+        f, t = _on_gpu("free_pages", free_pages, i32, dev), _on_gpu("tables", tables, i32, dev)
+        if free_pages.ndim != 1 or tables.ndim != 2 or tables.shape[0] != n:
+            raise ValueError(f"free_pages[m] and tables[{n}][max_pages] are needed: got {tuple(free_pages.shape)}, "
+                             f"{tuple(tables.shape)}")
+        max_tokens = int(max_tokens)
+        if max_tokens < 0:
+            raise ValueError(f"max_tokens {max_tokens} is negative")
+        out = PagePlan(*(torch.empty(k, dtype=i32, device=cached.device) for k in (n + 1, n, max_tokens, max_tokens, 2)))
+        _check(lib().gq_page_plan(c, m, n, page_size, f, free_pages.shape[0], t, tables.shape[1], out.q_start.data_ptr(),
+                                  out.ctx_lens.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(), max_tokens,
+                                  out.counts.data_ptr(), _stream(stream)))
+        _kept(stream, *out)
+        return out
+
+    def rope(self, q, k, positions, inv_freq, layout="half", mscale=1.0, q_out=None, k_out=None, stream=None):
+        """gq_rope: q [n][heads][head_dim] and k [n][kv_heads][head_dim] (or
+        None) turned by positions int32[n] with inv_freq float64[rot_dim / 2]
+        (rope_freqs, on the device); q_out / k_out may be q / k.  -> (q_out, k_out)"""
+        import torch
+        if layout not in _ROPE_LAYOUT:
+            raise ValueError(f"RoPE layout {layout!r}: one of {sorted(_ROPE_LAYOUT)} is needed")
+        dt, dev = _act(q), _device()
+        qp, qs = _rows("q", q, q)
+        n, nq, hd = q.shape
+        made = []
+        if q_out is None:
+            q_out = torch.empty((n, nq, hd), dtype=q.dtype, device=q.device)
+            made.append(q_out)
+        qo, qos = _rows("q_out", q_out, q, nq, hd)
+        kp = ko = None
+        ks = kos = nk = 0
+        if k is not None:
+            kp, ks = _rows("k", k, q, None, hd)
+            nk = k.shape[1]
+            if k_out is None:
+                k_out = torch.empty((n, nk, hd), dtype=q.dtype, device=q.device)
+                made.append(k_out)
+            ko, kos = _rows("k_out", k_out, q, nk, hd)
+            if k.shape[0] != n or k_out.shape[0] != n:
+                raise ValueError("q, k and k_out must have the same number of tokens")
+        if q_out.shape[0] != n:
+            raise ValueError("q and q_out must have the same number of tokens")
+        pp, fp = _on_gpu("positions", positions, torch.int32, dev, (n,)), _on_gpu("inv_freq", inv_freq, torch.float64, dev)
+        if q.get_device() != dev:
+            raise ValueError(f"q is on {q.device}, the current device is cuda:{dev}")
+        _check(lib().gq_rope(dt, _ROPE_LAYOUT[layout], n, hd, 2 * inv_freq.numel(), fp, mscale, pp, qp, qs, nq, qo, qos,
+                             kp, ks, nk, ko, kos, _stream(stream)))
+        _kept(stream, *made)
+        return q_out, k_out
+
+    def kv8_append(self, cache, k, v, slots, stream=None):
+        """gq_kv8_append: rows k, v [n][kv_heads][head_dim] at slots int32[n]."""
+        import torch
+        dev = _device()
+        c = _cache(cache, dev)
+        kp, ks = _rows("k", k, k, c.n_kv_heads, c.head_dim)
+        vp, vs = _rows("v", v, k, c.n_kv_heads, c.head_dim)
+        n = k.shape[0]
+        if v.shape[0] != n or k.get_device() != dev:
+            raise ValueError(f"k and v must have the same number of tokens, on cuda:{dev}")
+        _check(lib().gq_kv8_append(ctypes.byref(c), _act(k), kp, ks, vp, vs, _on_gpu("slots", slots, torch.int32, dev, (n,)),
+                                   n, _stream(stream)))
+
+    def kv8_read(self, cache, slots, dtype=None, stream=None):
+        """gq_kv8_read: the rows at slots int32[n] as values -> k, v
+        [n][kv_heads][head_dim] (float32, or dtype)."""
+        import torch
+        dev = _device()
+        c = _cache(cache, dev)
+        n = slots.shape[0]
+        sp = _on_gpu("slots", slots, torch.int32, dev, (n,))
+        k, v = (torch.empty((n, c.n_kv_heads, c.head_dim), dtype=dtype or torch.float32, device=slots.device) for _ in "kv")
+        _check(lib().gq_kv8_read(ctypes.byref(c), sp, n, _act(k), _ptr(k), _ptr(v), _stream(stream)))
+        _kept(stream, k, v)
+        return k, v
 
     def set_iq3xxs_grid(self, grid=None):
         if grid is None:

@@ -28,12 +28,14 @@ extern "C" {
 #define GQ_ENODEV (-6)   /* no gfx950 device / not initialised */
 
 /* GgmlType ids, the on-disk tensor type ids (src/types.rs:9-46). */
+#define GQ_TYPE_F32 0
 #define GQ_TYPE_F16 1
 #define GQ_TYPE_Q8_0 8
 #define GQ_TYPE_Q4_K 12
 #define GQ_TYPE_Q5_K 13
 #define GQ_TYPE_Q6_K 14
 #define GQ_TYPE_IQ3_XXS 18
+#define GQ_TYPE_BF16 30
 
 /* gq_gemm modes (batched prefill). */
 #define GQ_GEMM_BF16 0  /* weights dequantized to bf16, bf16 MFMA            */
@@ -245,6 +247,115 @@ int gq_model_prefill(gq_model *m, const int *tokens_host, int n, int pos, float 
  * receives the generated tokens (synchronous when non-NULL). */
 int gq_model_generate(gq_model *m, int token, int pos, int n_steps, int *tokens_host,
                       void *stream);
+
+/* ---- Many requests over a paged 8-bit KV cache --------------------------
+ * What a pass over many requests needs between its q, k, v products and its
+ * o product, as launches on device buffers: gq_page_plan, gq_rope,
+ * gq_kv8_append, gq_attn_kv8 (and gq_kv8_read to take a cache out).  The
+ * reference decodes one request over one contiguous cache (KvCache,
+ * src/model/mod.rs:605-700) with the half-layout RoPE of src/model/llama/
+ * cpu_path.rs:99-133, so these have no counterpart in it.
+ * All are asynchronous on `stream`, allocate nothing and may be captured;
+ * lengths and tables are read on the device, so a captured pass can be
+ * replayed for other requests within its bounds.  Activation types are
+ * GQ_TYPE_F32, GQ_TYPE_F16 and GQ_TYPE_BF16; sums, scales and angles are f32
+ * or wider.  Strides are in values, between tokens; a head's values are
+ * contiguous and heads follow each other.  Arguments are checked before
+ * anything is launched (GQ_EINVAL, GQ_EDTYPE).
+ *
+ * The cache: n_pages pages of page_size tokens (a multiple of 16, at most
+ * 256), head_dim 64 or 128.  A value is code * scale, codes -127 .. 127, one
+ * f32 scale for each page and KV head.  Slot s is offset s % page_size of page
+ * s / page_size; n_pages * page_size < 2^31.  Code buffers start at multiples
+ * of 16 bytes.  The caller owns the buffers; they need no initialisation. */
+typedef struct {
+  int n_pages, page_size, n_kv_heads, head_dim;
+  int8_t *k, *v;            /* dev [n_pages][n_kv_heads][page_size][head_dim] */
+  float *k_scale, *v_scale; /* dev [n_pages][n_kv_heads] */
+} gq_kv8;
+
+/* Where the tokens of a pass go.  Request i has cached[i] tokens in the cache
+ * and new[i] (>= 0) in this pass, its pages in order in tables[i][max_pages]
+ * (ceil(cached / page_size) of them held already).  Pages that it needs beyond
+ * those are taken from free_pages in order, requests in order, and written
+ * into its table; where free_pages ends the entries are -1.  With T = sum(new),
+ * token t of request r (tokens are request after request):
+ *   q_start[i]   sum of new[j], j < i  (n_requests + 1 values; the last is T)
+ *   ctx_lens[i]  cached[i] + new[i]
+ *   positions[t] cached[r] + t - q_start[r]
+ *   slots[t]     its slot, or -1: no page was left, max_pages are not enough, or the
+ *                slot does not fit an int
+ *   counts       {T, pages needed}  (more than n_free: the list was too short)
+ * Rows T .. max_tokens - 1 get position 0 and slot -1, so that a pass of fixed
+ * size leaves the cache alone there; of T > max_tokens tokens the first
+ * max_tokens are written.  Other entries of tables stay.  Negative lengths
+ * count as 0, and counts that pass INT_MAX stay there.  At most 4096 requests. */
+int gq_page_plan(const int *cached_dev, const int *new_dev, int n_requests, int page_size,
+                 const int *free_pages_dev, int n_free, int *tables_dev, int max_pages, int *q_start_dev,
+                 int *ctx_lens_dev, int *positions_dev, int *slots_dev, int max_tokens, int *counts_dev,
+                 void *stream);
+
+/* Rotary frequencies, on the host: inv_freq_host[rot_dim / 2] (radians a
+ * position) and the factor *mscale of the rotated values, for gq_rope.
+ *   GQ_ROPE_NONE    theta^(-2 i / rot_dim)
+ *   GQ_ROPE_LINEAR  those / factor
+ *   GQ_ROPE_YARN    dims that turn more than beta_fast times over orig_ctx
+ *                   positions as they are, less than beta_slow times / factor,
+ *                   a linear ramp over the dims between; mscale = attn_factor *
+ *                   (0.1 ln(factor) + 1)
+ *   GQ_ROPE_LLAMA3  more than high_freq turns over orig_ctx as they are, less than
+ *                   low_freq / factor, between them a mix linear in the turns
+ * and then each divided by freq_factors[i] if these are given (a GGUF file's
+ * rope_freqs.weight).  mscale is attn_factor otherwise. */
+#define GQ_ROPE_NONE 0
+#define GQ_ROPE_LINEAR 1
+#define GQ_ROPE_YARN 2
+#define GQ_ROPE_LLAMA3 3
+typedef struct {
+  int rot_dim, scaling;
+  double theta, factor, orig_ctx;
+  double beta_fast, beta_slow;  /* GQ_ROPE_YARN (32 and 1 in use) */
+  double low_freq, high_freq;   /* GQ_ROPE_LLAMA3 (1 and 4 in use) */
+  double attn_factor;           /* 1 */
+  const float *freq_factors;    /* host [rot_dim / 2], or NULL */
+} gq_rope_desc;
+int gq_rope_freqs(const gq_rope_desc *d, double *inv_freq_host, float *mscale);
+
+/* Rotary positions of q [n][n_heads][head_dim] and k [n][n_kv_heads][head_dim]
+ * (k may be NULL), token t at pos[t]: the first rot_dim (even) values of each
+ * head in pairs (i, i + rot_dim / 2) (GQ_ROPE_HALF) or (2 i, 2 i + 1)
+ * (GQ_ROPE_INTERLEAVED), pair i turned by pos * inv_freq[i], times mscale; the
+ * others as they are.  The angle is exact to 64 bits, at any position.  An
+ * output is its input's buffer (same stride) or overlaps nothing. */
+#define GQ_ROPE_HALF 0
+#define GQ_ROPE_INTERLEAVED 1
+int gq_rope(int dtype, int layout, int n, int head_dim, int rot_dim, const double *inv_freq_dev, float mscale,
+            const int *pos_dev, const void *q_dev, int64_t q_stride, int n_heads, void *q_out_dev,
+            int64_t q_out_stride, const void *k_dev, int64_t k_stride, int n_kv_heads, void *k_out_dev,
+            int64_t k_out_stride, void *stream);
+
+/* Rows k, v [n][n_kv_heads][head_dim] into the cache at slots[t]; rows whose
+ * slot is none of the cache's are skipped.  For each page and head that the
+ * call writes, with s the scale there (0 where a row goes to offset 0: it
+ * starts the page anew) and new rows x:
+ *   s' = max(s, max|x| / 127, 2^-60)
+ *   rows before the first new one: code' = rint(code * s / s') where s' > s
+ *   new rows:                      code  = rint(x / s')
+ * with the quotients exact and ties to even.  Rows behind them keep their codes.
+ * A value that is not finite makes the scale NaN until rows start the page
+ * anew; requests that do not see the page are not touched by it.
+ * The rows that a call writes into a page are neighbours in the call, in the
+ * order of their slots (gq_page_plan's are); what a page holds after a call
+ * that breaks this is not specified.  Buffers and strides are multiples of 16
+ * bytes. */
+int gq_kv8_append(const gq_kv8 *cache, int dtype, const void *k_dev, int64_t k_stride, const void *v_dev,
+                  int64_t v_stride, const int *slots_dev, int n, void *stream);
+
+/* The values at slots[t]: k_out, v_out [n][n_kv_heads][head_dim] (either may
+ * be NULL), zeros where the slot is none of the cache's.  What
+ * KvCache::read_up_to (src/model/mod.rs:682-700) is for the reference's. */
+int gq_kv8_read(const gq_kv8 *cache, const int *slots_dev, int n, int dtype, void *k_out_dev, void *v_out_dev,
+                void *stream);
 
 /* Wait for all work on `stream`. */
 int gq_sync(void *stream);
