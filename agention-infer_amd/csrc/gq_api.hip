@@ -1223,6 +1223,57 @@ int gq_kv8_read(const gq_kv8 *c, const int *slots_dev, int n, int dtype, void *k
   return launched("kv8 read", gq::launch_kv8_read(a, dtype, (hipStream_t)stream));
 }
 
+}  // extern "C"
+
+namespace {
+int check_attn(const gq_kv8 *c, int n_heads, int n_tokens, int n_requests, int max_new, int max_ctx) {
+  if (int rc = check_kv8(c)) return rc;
+  if (n_heads < 1 || n_heads % c->n_kv_heads)
+    return fail(GQ_EINVAL, "gq_attn_kv8: %d heads are no multiple of %d KV heads", n_heads, c->n_kv_heads);
+  if (n_tokens < 0 || n_requests < 0 || n_requests > 65535 || max_new < 0 || max_ctx < 0)
+    return fail(GQ_EINVAL, "gq_attn_kv8: %d tokens, %d requests (at most 65535), max_new %d, max_ctx %d", n_tokens, n_requests,
+                max_new, max_ctx);
+  if ((int64_t)max_new * (n_heads / c->n_kv_heads) > INT_MAX - 64)
+    return fail(GQ_EINVAL, "gq_attn_kv8: max_new %d of %d heads: too many rows", max_new, n_heads);
+  return GQ_OK;
+}
+}  // namespace
+
+extern "C" {
+size_t gq_attn_kv8_workspace(const gq_kv8 *c, int n_heads, int n_tokens, int n_requests, int max_new, int max_ctx) {
+  if (check_attn(c, n_heads, n_tokens, n_requests, max_new, max_ctx)) return 0;
+  const gq::AttnCut cut = gq::attn_cut(n_requests, c->n_kv_heads, n_heads / c->n_kv_heads, max_new, max_ctx);
+  return gq::attn_kv8_bytes(n_tokens, n_heads, c->head_dim, cut.parts);
+}
+
+int gq_attn_kv8(const gq_kv8 *c, int dtype, const void *q_dev, int64_t q_stride, int n_heads, int n_tokens,
+                const int *tables_dev, int max_pages, const int *q_start_dev, const int *ctx_lens_dev,
+                int n_requests, int max_new, int max_ctx, float scale, int window, void *out_dev,
+                int64_t out_stride, void *workspace_dev, size_t workspace_bytes, void *stream) {
+  if (int rc = check_attn(c, n_heads, n_tokens, n_requests, max_new, max_ctx)) return rc;
+  if (int rc = check_type("gq_attn_kv8", dtype)) return rc;
+  if (max_pages < 0 || window < 0) return fail(GQ_EINVAL, "gq_attn_kv8: max_pages %d, window %d", max_pages, window);
+  if (!std::isfinite(scale)) return fail(GQ_EINVAL, "gq_attn_kv8: scale %g", (double)scale);
+  if (n_tokens == 0 || n_requests == 0 || max_new == 0) return GQ_OK;
+  const int64_t w = (int64_t)n_heads * c->head_dim;
+  if (int rc = check_rows("q", q_dev, q_stride, w, dtype)) return rc;
+  if (int rc = check_rows("out", out_dev, out_stride, w, dtype)) return rc;
+  if ((max_pages && !tables_dev) || !q_start_dev || !ctx_lens_dev) return fail(GQ_EINVAL, "gq_attn_kv8: null buffer");
+  const int group = n_heads / c->n_kv_heads;
+  const gq::AttnCut cut = gq::attn_cut(n_requests, c->n_kv_heads, group, max_new, max_ctx);
+  const size_t need = gq::attn_kv8_bytes(n_tokens, n_heads, c->head_dim, cut.parts);
+  if (need && (!workspace_dev || workspace_bytes < need))
+    return fail(GQ_ESHORT, "gq_attn_kv8: workspace: need %zu bytes, have %zu", need, workspace_dev ? workspace_bytes : 0);
+  if (!aligned16(workspace_dev)) return fail(GQ_EINVAL, "gq_attn_kv8: the workspace must start at a multiple of 16 bytes");
+  if ((int64_t)cut.tiles * cut.parts > INT_MAX) return fail(GQ_EINVAL, "gq_attn_kv8: too many rows by keys in one call");
+  if (int rc = ensure_init()) return rc;
+  const gq::AttnArgs a{c->k,       c->v,         c->k_scale,    c->v_scale,    q_dev,      out_dev,        q_stride, out_stride,
+                       tables_dev, q_start_dev,  ctx_lens_dev,  (float *)workspace_dev, scale, c->n_pages, c->page_size,
+                       c->n_kv_heads, group,     n_tokens,      n_requests,    max_pages,  window,         max_new,  max_ctx,
+                       cut.split,  cut.parts};
+  return launched("attention", gq::launch_attn_kv8(a, dtype, c->head_dim, cut.tiles, (hipStream_t)stream));
+}
+
 int gq_sync(void *stream) {
   HIP_TRY(hipStreamSynchronize((hipStream_t)stream));
   return GQ_OK;

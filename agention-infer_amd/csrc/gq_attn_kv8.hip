@@ -1,0 +1,324 @@
+// gq_attn_kv8.hip -- attention of a pass's query rows over the paged 8-bit
+// cache (its layout: gq_paged.hip).
+//
+//   s_t = scale q . (c^K_t ks_t),  p_t = e^(s_t) over the keys t that the row
+//   sees,  o = sum_t p_t c^V_t vs_t / sum_t p_t
+// with codes c, and one scale ks, vs for each page and KV head.  Scores are kept
+// in base 2 with the V scale in them, z_t = log2(e) s_t + log2 vs_t, so that
+// with M the largest z so far
+//   w_t = 2^(z_t - M + 15),  O = sum_t w_t c^V_t,  l = sum_t w_t / vs_t,  o = O / l
+// takes the scale of each page for no more than an fma per score and one per
+// sum.  The 15 puts the weights into the upper range of f16, so that those down
+// to 2^-29 of the largest keep all of its bits.
+//
+// Both products run on v_mfma_f32_16x16x32_f16: codes are exact in f16; q is
+// scaled by a power of two and split into f16 hi + lo, as are the weights, for
+// f32 activations (22 bits each), and rounded to one f16 for 16-bit ones (11
+// bits: their own rounding is as large).
+#include <type_traits>
+
+#include "gq_device.h"
+#include "gq_internal.h"
+#include "gq_paged.h"
+
+namespace gq {
+
+typedef _Float16 a8_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 a8_f16x2 __attribute__((ext_vector_type(2)));
+typedef float a8_f32x4 __attribute__((ext_vector_type(4)));
+
+// f16 of the two codes whose bytes (biased by 128) are bytes 0 and 2 of x:
+// 0x6400 | u is 1024 + u exactly.
+__device__ __forceinline__ uint32_t f16_of_biased(uint32_t x) {
+  const a8_f16x2 b = __builtin_bit_cast(a8_f16x2, x) - a8_f16x2{(_Float16)1152.f, (_Float16)1152.f};
+  return __builtin_bit_cast(uint32_t, b);
+}
+// Four codes of a dword in order.
+__device__ __forceinline__ void f16_of_dword(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  lo = f16_of_biased(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+  hi = f16_of_biased(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+}
+// Byte B of dwords a and b (already biased).
+template <int B>
+__device__ __forceinline__ uint32_t f16_of_bytes(uint32_t a, uint32_t b) {
+  return f16_of_biased(__builtin_amdgcn_perm(b, a, 0x0c040c00u + 0x00010001u * B) | 0x64006400u);
+}
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ------------------------------------------------------------- row tiles
+// A block is one tile of 16 query rows of a (request, KV head) over one part
+// of its keys.  Rows are the request's tokens by the KV head's query heads, so
+// the heads that share K and V, and a draft's tokens, share one read of them.
+// Its 4 waves take chunks of 64 keys in turn, each with its own M, l, O, and
+// meet once at the end; nothing goes through LDS before that:
+//   S^T = K . q^T  A = 16 keys x 32 dims.  Lane (m = lane % 16, g = lane / 16)
+//         takes row m's bytes [HD/4 g, HD/4 (g + 1)), so a key's row is read by
+//         4 lanes in 16-byte loads; step ks multiplies the 8 of them at 8 ks,
+//         and q's fragments hold the same dims.
+//   O^T = V^T . P^T  B = the lane's own weights (keys 16 t0 + 4 g + j, j < 4,
+//         and 16 t1 + 4 g + j - 4), A = V^T in that key order: the lane loads
+//         HD/16 bytes at HD/16 m of these 8 rows, and byte e of the 8 is row m
+//         of tile e, so tile e of O^T holds dims HD/16 m + e.
+constexpr int ROWS_THREADS = 256;
+template <class T, int HD>
+__global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
+  constexpr bool SPLIT = std::is_same<T, float>::value;  // hi + lo operands
+  constexpr int KS = HD / 32, KV = HD / 64, DPL = HD / 16;
+  constexpr int NW = ROWS_THREADS / 64, LD = HD + 4;
+  __shared__ __align__(16) float so[NW][16][LD];
+  __shared__ float sm[NW][16], sl[NW][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int m = lane & 15, g = lane >> 4;
+  const int tile = blockIdx.x / a.parts, part = blockIdx.x % a.parts, kh = blockIdx.y, b = blockIdx.z;
+  const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
+  const int rows = min((int64_t)rq.fresh * a.group - (int64_t)tile * 16, (int64_t)16);
+  if (rows <= 0) return;
+  const int row0 = tile * 16;
+  const AttnKeys ak = attn_keys(rq, row0 / a.group, (row0 + rows - 1) / a.group, a.window);
+  const int nparts = attn_parts(ak, a.split);
+  if (part >= nparts) return;
+  const int64_t klo = (int64_t)ak.lo + (int64_t)part * a.split;
+  const int khi = (int)min((int64_t)ak.hi, klo + a.split);
+  const int nh = a.n_kv * a.group;
+
+  // q: row m's values of this lane's dims, scaled to 2^14 .. 2^15
+  const int myrow = row0 + min(m, rows - 1), mytok = myrow / a.group, myhead = kh * a.group + myrow % a.group;
+  const T *qp = (const T *)a.q + (int64_t)(rq.start + mytok) * a.q_stride + (int64_t)myhead * HD + (HD / 4) * g;
+  float qv[HD / 4];
+  float qm = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 4; i++) {
+    qv[i] = (float)qp[i];
+    qm = fmaxf(qm, fabsf(qv[i]));
+  }
+  qm = lane_groups_max(qm);
+  int ex = 0;
+  (void)frexpf(qm, &ex);
+  const float up = qm > 0.f ? ldexpf(1.f, min(15 - ex, 126)) : 1.f;
+  const float qf = a.scale * 1.4426950408889634f / up;
+  a8_f16x8 qh[KS], ql[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float x = qv[8 * ks + j] * up;
+      qh[ks][j] = (_Float16)x;
+      if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
+    }
+  // keys that row m sees: (see_lo, see_hi]
+  const int see_hi = m < rows ? rq.first + mytok : -1;
+  const int64_t see_lo = a.window ? (int64_t)see_hi - a.window : -1;
+
+  float M = -INFINITY, l = 0.f;
+  a8_f32x4 O[DPL];
+#pragma unroll
+  for (int e = 0; e < DPL; e++) O[e] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
+  const int *table = a.tables + (int64_t)b * a.wide;
+
+  for (int64_t k0 = klo + 64 * wave; k0 < khi; k0 += 64 * NW) {
+    uint4 kf[4][KV];
+    uint32_t vf[4][4][DPL / 4];
+    float ksc[4], vsc[4];
+    bool ok[4];
+    int pj = (int)(k0 / a.page), off = (int)(k0 % a.page);
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      int id = k0 + 16 * t < khi ? table[pj] : -1;
+      ok[t] = id >= 0 && id < a.n_pages;
+      if (!ok[t]) id = 0;  // (its rows are read and not used)
+      const int64_t ph = (int64_t)id * a.n_kv + kh;
+      ksc[t] = a.ks[ph];
+      vsc[t] = a.vs[ph];
+      const int8_t *kp = a.kc + (ph * a.page + off + m) * HD + (HD / 4) * g;
+      const int8_t *vp = a.vc + (ph * a.page + off + 4 * g) * HD + DPL * m;
+#pragma unroll
+      for (int i = 0; i < KV; i++) kf[t][i] = *(const uint4 *)(kp + 16 * i);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < DPL / 4; i++) vf[t][j][i] = *(const uint32_t *)(vp + j * HD + 4 * i);
+      off += 16;
+      if (off == a.page) {
+        off = 0;
+        pj++;
+      }
+    }
+    float z[4][4], ivs[4];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      a8_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const uint4 w = kf[t][ks / 2];
+        uint4 f;
+        f16_of_dword(ks & 1 ? w.z : w.x, f.x, f.y);
+        f16_of_dword(ks & 1 ? w.w : w.y, f.z, f.w);
+        const a8_f16x8 k8 = __builtin_bit_cast(a8_f16x8, f);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[ks], acc, 0, 0, 0);
+        if (SPLIT) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[ks], acc, 0, 0, 0);
+      }
+      const float f = ksc[t] * qf, lv = log2f(vsc[t]);
+      ivs[t] = 1.f / vsc[t];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int64_t key = k0 + 16 * t + 4 * g + i;
+        const bool sees = ok[t] && key <= see_hi && key > see_lo;
+        z[t][i] = sees ? fmaf(acc[i], f, lv) : -INFINITY;
+        mx = fmaxf(mx, z[t][i]);
+      }
+    }
+    const float Mn = fmaxf(M, lane_groups_max(mx));
+    const float alpha = M == -INFINITY ? 0.f : exp2_raw(M - Mn), base = Mn == -INFINITY ? 0.f : Mn - 15.f;
+    M = Mn;
+    l *= alpha;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float p = exp2_raw(z[t][i] - base);
+        z[t][i] = p;
+        // (a key that is not seen adds nothing, whatever its page's scale)
+        l = fmaf(p, p == 0.f ? 0.f : ivs[t], l);
+      }
+#pragma unroll
+    for (int e = 0; e < DPL; e++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) O[e][i] *= alpha;
+#pragma unroll
+    for (int st = 0; st < 2; st++) {
+      a8_f16x8 ph8, pl8;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float p = z[2 * st + j / 4][j & 3];
+        ph8[j] = (_Float16)p;
+        if (SPLIT) pl8[j] = (_Float16)(p - (float)ph8[j]);
+      }
+#pragma unroll
+      for (int i = 0; i < DPL / 4; i++) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = vf[2 * st + j / 4][j & 3][i] ^ 0x80808080u;
+        auto step = [&](a8_f32x4 &o, uint4 f) {
+          const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, f);
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph8, o, 0, 0, 0);
+          if (SPLIT) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl8, o, 0, 0, 0);
+        };
+        step(O[4 * i + 0], make_uint4(f16_of_bytes<0>(w[0], w[1]), f16_of_bytes<0>(w[2], w[3]),
+                                      f16_of_bytes<0>(w[4], w[5]), f16_of_bytes<0>(w[6], w[7])));
+        step(O[4 * i + 1], make_uint4(f16_of_bytes<1>(w[0], w[1]), f16_of_bytes<1>(w[2], w[3]),
+                                      f16_of_bytes<1>(w[4], w[5]), f16_of_bytes<1>(w[6], w[7])));
+        step(O[4 * i + 2], make_uint4(f16_of_bytes<2>(w[0], w[1]), f16_of_bytes<2>(w[2], w[3]),
+                                      f16_of_bytes<2>(w[4], w[5]), f16_of_bytes<2>(w[6], w[7])));
+        step(O[4 * i + 3], make_uint4(f16_of_bytes<3>(w[0], w[1]), f16_of_bytes<3>(w[2], w[3]),
+                                      f16_of_bytes<3>(w[4], w[5]), f16_of_bytes<3>(w[6], w[7])));
+      }
+    }
+  }
+
+  // The waves' results, each to the largest M of its row.
+  l = lane_groups_sum(l);
+  if (g == 0) {
+    sm[wave][m] = M;
+    sl[wave][m] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {  // dims DPL (4 g + i) + e of row m
+    float *p = &so[wave][m][DPL * (4 * g + i)];
+#pragma unroll
+    for (int e = 0; e < DPL; e += 4) *(float4 *)(p + e) = make_float4(O[e][i], O[e + 1][i], O[e + 2][i], O[e + 3][i]);
+  }
+  __syncthreads();
+  const int r = tid >> 4, d = (tid & 15) * DPL;
+  if (r >= rows) return;
+  float Mr = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; w++) Mr = fmaxf(Mr, sm[w][r]);
+  float lr = 0.f, o[DPL] = {};
+#pragma unroll
+  for (int w = 0; w < NW; w++) {
+    const float c = sm[w][r] == -INFINITY ? 0.f : exp2_raw(sm[w][r] - Mr);
+    lr = fmaf(sl[w][r], c, lr);
+#pragma unroll
+    for (int e = 0; e < DPL; e++) o[e] = fmaf(so[w][r][d + e], c, o[e]);
+  }
+  const int tok = rq.start + (row0 + r) / a.group, head = kh * a.group + (row0 + r) % a.group;
+  if (nparts > 1) {
+    float *p = a.part + (((int64_t)tok * nh + head) * a.parts + part) * LD;
+#pragma unroll
+    for (int e = 0; e < DPL; e += 4) *(float4 *)(p + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+    if (d == 0) *(float2 *)(p + HD) = make_float2(Mr, lr);
+    return;
+  }
+  T *op = (T *)a.out + (int64_t)tok * a.out_stride + (int64_t)head * HD + d;
+#pragma unroll
+  for (int e = 0; e < DPL; e++) op[e] = (T)(lr == 0.f ? 0.f : o[e] / lr);
+}
+
+// The parts of a row joined: o = sum_p O_p 2^(M_p - M) / sum_p l_p 2^(M_p - M).
+// A wave is one row; rows of one part are written already.
+constexpr int JOIN_THREADS = 256;
+template <class T, int HD>
+__global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
+  constexpr int LD = HD + 4, DPL = HD / 64;
+  const int lane = threadIdx.x & 63, kh = blockIdx.y, b = blockIdx.z;
+  const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
+  const int64_t row = (int64_t)blockIdx.x * (JOIN_THREADS / 64) + (threadIdx.x >> 6);
+  const int64_t all = (int64_t)rq.fresh * a.group;
+  if (row >= all) return;
+  const int row0 = (int)(row / 16 * 16);  // of its tile
+  const AttnKeys ak = attn_keys(rq, row0 / a.group, (int)(min((int64_t)row0 + 16, all) - 1) / a.group, a.window);
+  const int n = attn_parts(ak, a.split);
+  if (n == 1) return;
+  const int nh = a.n_kv * a.group, tok = rq.start + (int)(row / a.group), head = kh * a.group + (int)(row % a.group);
+  const float *p = a.part + ((int64_t)tok * nh + head) * a.parts * LD;
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 64) M = fmaxf(M, p[(int64_t)i * LD + HD]);
+  M = wave_max(M);
+  float l = 0.f, o[DPL] = {};
+  for (int i = 0; i < n; i++) {
+    const float *pi = p + (int64_t)i * LD;
+    const float c = pi[HD] == -INFINITY ? 0.f : exp2_raw(pi[HD] - M);
+    l = fmaf(pi[HD + 1], c, l);
+#pragma unroll
+    for (int e = 0; e < DPL; e++) o[e] = fmaf(pi[DPL * lane + e], c, o[e]);
+  }
+  T *op = (T *)a.out + (int64_t)tok * a.out_stride + (int64_t)head * HD + DPL * lane;
+#pragma unroll
+  for (int e = 0; e < DPL; e++) op[e] = (T)(l == 0.f ? 0.f : o[e] / l);
+}
+
+size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, int parts) {
+  return parts > 1 ? (size_t)n_tokens * n_heads * parts * (hd + 4) * sizeof(float) : 0;
+}
+
+template <class T, int HD>
+static void attn_launch(const AttnArgs &a, int tiles, hipStream_t st) {
+  hipLaunchKernelGGL((k_attn_kv8_rows<T, HD>), dim3(tiles * a.parts, a.n_kv, a.n_requests), dim3(ROWS_THREADS), 0, st, a);
+  if (a.parts > 1) {
+    const int64_t rows = (int64_t)a.max_new * a.group;
+    hipLaunchKernelGGL((k_attn_kv8_join<T, HD>), dim3((unsigned)((rows + 3) / 4), a.n_kv, a.n_requests), dim3(JOIN_THREADS), 0,
+                       st, a);
+  }
+}
+
+hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, int tiles, hipStream_t st) {
+  auto go = [&](auto zero) {
+    typedef decltype(zero) T;
+    if (hd == 64)
+      attn_launch<T, 64>(a, tiles, st);
+    else
+      attn_launch<T, 128>(a, tiles, st);
+  };
+  if (dtype == T_F32)
+    go(0.f);
+  else if (dtype == T_F16)
+    go((_Float16)0);
+  else
+    go((__bf16)0);
+  return hipGetLastError();
+}
+
+}  // namespace gq

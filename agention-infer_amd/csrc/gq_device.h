@@ -245,4 +245,20 @@ __device__ __forceinline__ float wave_sum(float x) {
   return wave_reduce(x, [](float a, float b) { return a + b; });
 }
 
+// Max / sum of x over the 4 lane groups (lanes 16 apart) of a wave, the
+// same value in every lane (gfx950 lane swaps; each combination is
+// symmetric, so every lane computes the identical bits).
+__device__ __forceinline__ float lane_groups_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float lane_groups_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 }  // namespace gq

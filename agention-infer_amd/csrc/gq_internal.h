@@ -329,4 +329,20 @@ struct ReadArgs {
 };
 hipError_t launch_kv8_read(const ReadArgs &a, int dtype, hipStream_t st);
 
+// Attention over the cache (gq_attn_kv8.hip).
+struct AttnArgs {
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  const void *q;
+  void *out;
+  int64_t q_stride, out_stride;
+  const int *tables, *q_start, *ctx_lens;
+  float *part;  // [n_tokens][n_heads][parts][hd + 4]: O, then m, l
+  float scale;
+  int n_pages, page, n_kv, group, n_tokens, n_requests, wide, window;
+  int max_new, max_ctx, split, parts;
+};
+size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, int parts);
+hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, int tiles, hipStream_t st);
+
 }  // namespace gq

@@ -49,4 +49,66 @@ GQ_HD int owner_of(const int *at, int n, int v) {
   return lo;
 }
 
+// ------------------------------------------------------------- attention
+// A request of a pass: its rows are tokens [start, start + fresh) of the
+// pass, token i at position first + i (first < 0: ctx says less than its own
+// tokens, the first of which then see nothing); keys are positions < keys.
+// Whatever the device's q_start and ctx_lens hold, rows stay within the pass
+// and keys within the request's table and the call's max_ctx.
+struct AttnRequest {
+  int start, fresh, first, keys;
+};
+GQ_HD AttnRequest attn_request(int s, int e, int ctx, int n_tokens, int wide, int page, int max_ctx) {
+  AttnRequest r;
+  r.start = s < 0 ? 0 : s > n_tokens ? n_tokens : s;
+  const int end = e < r.start ? r.start : e > n_tokens ? n_tokens : e;
+  r.fresh = end - r.start;
+  const int c = not_negative(ctx);
+  r.first = c - r.fresh;
+  const int64_t held = (int64_t)wide * page, cap = held < max_ctx ? held : max_ctx;
+  r.keys = c < cap ? c : (int)cap;
+  return r;
+}
+
+// The keys that any of tokens i0 .. i1 of the request sees: [lo, hi), lo a
+// multiple of ATTN_CHUNK (hi <= lo: none).
+constexpr int ATTN_CHUNK = 64;
+struct AttnKeys {
+  int lo, hi;
+};
+GQ_HD AttnKeys attn_keys(const AttnRequest &r, int i0, int i1, int window) {
+  AttnKeys k;
+  const int last = r.first + i1 + 1;
+  k.hi = last < r.keys ? last : r.keys;
+  const int64_t from = window ? (int64_t)r.first + i0 - window + 1 : 0;
+  k.lo = from <= 0 ? 0 : (int)(from / ATTN_CHUNK * ATTN_CHUNK);
+  return k;
+}
+
+// Parts that the keys of a tile are cut into, `split` keys each (at least one
+// part, which may be empty).
+GQ_HD int attn_parts(const AttnKeys &k, int split) {
+  return k.hi <= k.lo ? 1 : (k.hi - k.lo - 1) / split + 1;
+}
+
+// How a call is cut: tiles of 16 rows (rows of a request: tokens by query
+// heads of one KV head), its keys in parts of `split`, at most `parts` of them.
+struct AttnCut {
+  int tiles, split, parts;
+};
+inline AttnCut attn_cut(int n_requests, int n_kv_heads, int group, int max_new, int max_ctx) {
+  AttnCut c;
+  c.tiles = (int)(((int64_t)max_new * group + 15) / 16);
+  const int64_t blocks = (int64_t)c.tiles * n_kv_heads * n_requests;
+  const int64_t most = ((int64_t)max_ctx + 255) / 256, want = blocks ? 4096 / blocks : 1;
+  const int64_t n = want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most;
+  int64_t split = (((int64_t)max_ctx + n - 1) / n + 255) / 256 * 256;
+  if (split < 256) split = 256;
+  if (split > (1 << 30)) split = 1 << 30;
+  c.split = (int)split;
+  c.parts = (int)(((int64_t)max_ctx + split - 1) / split);
+  if (c.parts < 1) c.parts = 1;
+  return c;
+}
+
 }  // namespace gq

@@ -267,22 +267,6 @@ __global__ __launch_bounds__(256) void k_kv_q8_to_f16(const int8_t *kc, const in
   vf[i] = __half_as_ushort(__float2half_rn((float)vc[i] * __half2float(__ushort_as_half(vsc[sb]))));
 }
 
-// Max / sum of x over the 4 lane groups (lanes 16 apart) of a wave, the
-// same value in every lane (gfx950 lane swaps; each combination is
-// symmetric, so every lane computes the identical bits).
-__device__ __forceinline__ float lane_groups_max(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float lane_groups_sum(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 constexpr int PF_Q = 64;  // queries per block
 typedef short pf16x4s_t __attribute__((ext_vector_type(4)));
 typedef short pf16x8s_t __attribute__((ext_vector_type(8)));

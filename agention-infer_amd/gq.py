@@ -70,6 +70,8 @@ SIGNATURES = {
     "gq_rope": (_I, [_I, _I, _I, _I, _I, _P, ctypes.c_float, _P, _P, _L, _I, _P, _L, _P, _L, _I, _P, _L, _P]),
     "gq_kv8_append": (_I, [_P, _I, _P, _L, _P, _L, _P, _I, _P]),
     "gq_kv8_read": (_I, [_P, _P, _I, _I, _P, _P, _P]),
+    "gq_attn_kv8_workspace": (_SZ, [_P, _I, _I, _I, _I, _I]),
+    "gq_attn_kv8": (_I, [_P, _I, _P, _L, _I, _I, _P, _I, _P, _P, _I, _I, _I, ctypes.c_float, _I, _P, _L, _P, _SZ, _P]),
     "gq_moe_ffn_noalloc": (_I, [_P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
 }
 
@@ -534,6 +536,43 @@ class HipBackend:
         _check(lib().gq_kv8_read(ctypes.byref(c), sp, n, _act(k), _ptr(k), _ptr(v), _stream(stream)))
         _kept(stream, k, v)
         return k, v
+
+    def attn_kv8(self, q, cache, tables, q_start, ctx_lens, max_new, max_ctx, scale=None, window=0, out=None,
+                 workspace=None, stream=None):
+        """gq_attn_kv8: q [n][heads][head_dim] of the pass's rows (request i's
+        are q_start[i] .. q_start[i + 1] - 1), tables int32[n_requests][max_pages],
+        ctx_lens int32[n_requests]; scale 1 / sqrt(head_dim) by default -> out
+        like q.  Rows of no request are left as `out` has them.  workspace: a
+        uint8 tensor to use instead of a new one where the call needs any."""
+        import torch
+        dt, dev, i32 = _act(q), _device(), torch.int32
+        c = _cache(cache, dev)
+        qp, qs = _rows("q", q, q, None, c.head_dim)
+        n, nh, hd = q.shape
+        nr = ctx_lens.shape[0]
+        tp = _on_gpu("tables", tables, i32, dev)
+        if tables.ndim != 2 or tables.shape[0] != nr:
+            raise ValueError(f"tables[{nr}][max_pages] are needed: got {tuple(tables.shape)}")
+        sp, cp = _on_gpu("q_start", q_start, i32, dev, (nr + 1,)), _on_gpu("ctx_lens", ctx_lens, i32, dev, (nr,))
+        if q.get_device() != dev:
+            raise ValueError(f"q is on {q.device}, the current device is cuda:{dev}")
+        L, cr, made = lib(), ctypes.byref(c), []
+        if out is None:
+            out = torch.empty((n, nh, hd), dtype=q.dtype, device=q.device)
+            made.append(out)
+        op, os_ = _rows("out", out, q, nh, hd)
+        if out.shape[0] != n:
+            raise ValueError("q and out must have the same number of tokens")
+        if workspace is None:
+            need = L.gq_attn_kv8_workspace(cr, nh, n, nr, max_new, max_ctx)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+                made.append(workspace)
+        wp, wb = (None, 0) if workspace is None else (_on_gpu("workspace", workspace, torch.uint8, dev), workspace.numel())
+        _check(L.gq_attn_kv8(cr, dt, qp, qs, nh, n, tp, tables.shape[1], sp, cp, nr, max_new, max_ctx,
+                             hd ** -0.5 if scale is None else scale, window, op, os_, wp, wb, _stream(stream)))
+        _kept(stream, *made)
+        return out
 
     def set_iq3xxs_grid(self, grid=None):
         if grid is None:

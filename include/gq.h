@@ -357,6 +357,33 @@ int gq_kv8_append(const gq_kv8 *cache, int dtype, const void *k_dev, int64_t k_s
 int gq_kv8_read(const gq_kv8 *cache, const int *slots_dev, int n, int dtype, void *k_out_dev, void *v_out_dev,
                 void *stream);
 
+/* Attention of a pass's rows q [n_tokens][n_heads][head_dim] over the cache:
+ * request i has rows q_start[i] .. q_start[i + 1] - 1, the last of them at
+ * position ctx_lens[i] - 1, and the pages tables[i][max_pages]; query head h
+ * reads KV head h / (n_heads / n_kv_heads).  Row at position p sees the keys
+ * at positions <= p, with a window > 0 of them only those > p - window, on
+ * pages that the cache has (an entry < 0 or >= n_pages hides its keys):
+ *   out = sum_t e^(scale q.k_t) v_t / sum_t e^(scale q.k_t),
+ * zeros for a row that sees nothing.  Keys that a row does not see have no
+ * effect on it, whatever they hold.  out has q's type; sums and the softmax
+ * are f32, products carry 22 bits of f32 q and of the weights (11 for 16-bit
+ * types).  The cache's scales are as gq_kv8_append leaves them (>= 2^-60).
+ * max_new and max_ctx bound the rows and positions of a request: rows past
+ * max_new are not computed, keys past max_ctx (or the table) not seen.  Rows
+ * that belong to no request, behind q_start[n_requests] among them, are left
+ * as they are.  At most 65535 requests; a new row's own k and v are in the
+ * cache before the call.  Buffers and strides are multiples of 16 bytes; out
+ * overlaps nothing.
+ * The workspace is the caller's: gq_attn_kv8_workspace bytes (0 where none is
+ * needed or the sizes are refused) at a multiple of 16, for one call at a time
+ * (captured calls that are replayed side by side need their own). */
+size_t gq_attn_kv8_workspace(const gq_kv8 *cache, int n_heads, int n_tokens, int n_requests, int max_new,
+                             int max_ctx);
+int gq_attn_kv8(const gq_kv8 *cache, int dtype, const void *q_dev, int64_t q_stride, int n_heads, int n_tokens,
+                const int *tables_dev, int max_pages, const int *q_start_dev, const int *ctx_lens_dev,
+                int n_requests, int max_new, int max_ctx, float scale, int window, void *out_dev,
+                int64_t out_stride, void *workspace_dev, size_t workspace_bytes, void *stream);
+
 /* Wait for all work on `stream`. */
 int gq_sync(void *stream);
 

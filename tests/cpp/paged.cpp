@@ -3,6 +3,9 @@
 //   pages TOKENS P WIDE   ->  pages_of
 //   slot ID P OFF         ->  slot_of
 //   owner N V AT0 .. ATN  ->  owner_of
+//   req S E CTX N WIDE PAGE MAXCTX  ->  start fresh first keys of attn_request
+//   keys FRESH FIRST KEYS I0 I1 WINDOW SPLIT  ->  lo hi of attn_keys, attn_parts
+//   cut REQUESTS KV GROUP MAXNEW MAXCTX  ->  tiles split parts of attn_cut
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -24,6 +27,22 @@ int main() {
       for (int &v : at)
         if (std::scanf("%d", &v) != 1) return 1;
       std::printf("%d\n", gq::owner_of(at.data(), a, b));
+    } else if (!std::strcmp(what, "req")) {
+      int s, e, ctx, n, wide, page, most;
+      if (std::scanf("%d %d %d %d %d %d %d", &s, &e, &ctx, &n, &wide, &page, &most) != 7) return 1;
+      const gq::AttnRequest r = gq::attn_request(s, e, ctx, n, wide, page, most);
+      std::printf("%d %d %d %d\n", r.start, r.fresh, r.first, r.keys);
+    } else if (!std::strcmp(what, "keys")) {
+      gq::AttnRequest r{};
+      int i0, i1, window, split;
+      if (std::scanf("%d %d %d %d %d %d %d", &r.fresh, &r.first, &r.keys, &i0, &i1, &window, &split) != 7) return 1;
+      const gq::AttnKeys k = gq::attn_keys(r, i0, i1, window);
+      std::printf("%d %d %d\n", k.lo, k.hi, gq::attn_parts(k, split));
+    } else if (!std::strcmp(what, "cut")) {
+      int nr, kv, group, fresh, ctx;
+      if (std::scanf("%d %d %d %d %d", &nr, &kv, &group, &fresh, &ctx) != 5) return 1;
+      const gq::AttnCut t = gq::attn_cut(nr, kv, group, fresh, ctx);
+      std::printf("%d %d %d\n", t.tiles, t.split, t.parts);
     } else {
       return 1;
     }

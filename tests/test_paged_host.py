@@ -61,6 +61,8 @@ def test_no_tokens_are_no_work():
     assert gq.lib().gq_rope(*dict(ROPE, n=0).values()) == 0
     assert gq.lib().gq_kv8_append(kv8(), gq.F32, P, 128, P, 128, P, 0, None) == 0
     assert gq.lib().gq_kv8_read(kv8(), P, 0, gq.F32, P, P, None) == 0
+    for none in ("n", "nr", "max_new"):
+        assert gq.lib().gq_attn_kv8(kv8(), *dict(ATTN, **{none: 0}).values()) == 0
 
 
 CACHES = [(dict(page=20), "page_size 20"), (dict(page=512), "page_size 512"), (dict(hd=96), "head_dim 96"),
@@ -75,6 +77,27 @@ def test_bad_caches_are_refused(change, text):
     c = kv8(**change)
     refused(gq.lib().gq_kv8_append(c, gq.F32, P, 4 << 20, P, 4 << 20, P, 2, None), EINVAL, text)
     refused(gq.lib().gq_kv8_read(c, P, 2, gq.F32, P, P, None), EINVAL, text)
+    assert gq.lib().gq_attn_kv8_workspace(c, 4, 8, 2, 4, 64) == 0
+    refused(gq.lib().gq_attn_kv8(c, *ATTN.values()), EINVAL, text)
+
+
+ATTN = dict(dtype=gq.F32, q=P, qs=256, nh=4, n=8, tables=P, wide=4, q_start=P, ctx=P, nr=2, max_new=4, max_ctx=64, scale=0.1,
+            window=0, out=2 * P, os=256, ws=P, wb=1 << 30, stream=None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(dtype=12), EDTYPE, "Q4_K"), (dict(nh=3), EINVAL, "3 heads"), (dict(nh=0), EINVAL, "0 heads"),
+    (dict(n=-1), EINVAL, "-1 tokens"), (dict(nr=-1), EINVAL, "-1 requests"), (dict(nr=65536), EINVAL, "at most 65535"),
+    (dict(max_new=-1), EINVAL, "max_new -1"), (dict(max_ctx=-1), EINVAL, "max_ctx -1"), (dict(wide=-1), EINVAL, "max_pages -1"),
+    (dict(window=-1), EINVAL, "window -1"), (dict(scale=math.inf), EINVAL, "scale"), (dict(scale=math.nan), EINVAL, "scale"),
+    (dict(max_new=2**30), EINVAL, "too many rows"), (dict(qs=255), EINVAL, "q: rows"), (dict(os=128), EINVAL, "out: rows"),
+    (dict(qs=257), EINVAL, "multiples of 16"), (dict(os=258), EINVAL, "multiples of 16"), (dict(q=P + 4), EINVAL, "multiples of 16"),
+    (dict(out=P + 8), EINVAL, "multiples of 16"), (dict(q=None), EINVAL, "null q"), (dict(out=None), EINVAL, "null out"),
+    (dict(tables=None), EINVAL, "null"), (dict(q_start=None), EINVAL, "null"), (dict(ctx=None), EINVAL, "null"),
+    (dict(max_ctx=9000, ws=None), -3, "have 0"), (dict(max_ctx=9000, wb=15), -3, "have 15"),
+    (dict(ws=P + 8), EINVAL, "workspace must start")])
+def test_attention_refuses(change, code, text):
+    refused(gq.lib().gq_attn_kv8(kv8(), *dict(ATTN, **change).values()), code, text)
 
 
 @pytest.mark.parametrize("dtype,k,ks,v,vs,slots,n,code,text", [
@@ -193,3 +216,53 @@ def test_owner(ask):
             lines.append(f"owner {n} {v} " + " ".join(map(str, at)))
             want.append(int(np.searchsorted(at[1:], v, side="right")))
     assert [r[0] for r in ask(lines)] == want
+
+
+def test_attention_rows_and_keys_stay_inside(ask):
+    """Whatever the device's lengths hold: rows within the pass, keys within
+    the table and the bound; sane lengths give the request's own."""
+    rng = np.random.default_rng(2)
+    wild = [-2**31, -5, 0, 3, 40, 2**31 - 1]
+    cases = [(int(rng.choice(wild)), int(rng.choice(wild)), int(rng.choice(wild)), int(rng.choice([0, 1, 9, 2**31 - 1])),
+              int(rng.choice([0, 1, 7, 2**23])), int(rng.choice([16, 48, 256])), int(rng.choice([0, 5, 700, 2**31 - 1])))
+             for _ in range(400)]
+    for (s, e, ctx, n, wide, page, most), (start, fresh, first, keys) in zip(
+            cases, ask(["req " + " ".join(map(str, c)) for c in cases])):
+        assert 0 <= start <= n and fresh >= 0 and start + fresh <= n
+        assert 0 <= keys <= min(wide * page, most, max(ctx, 0)) and first == max(ctx, 0) - fresh
+    assert ask(["req 4 9 30 20 9 16 64", "req 4 9 30 20 1 16 64", "req 4 9 30 20 9 16 25"]) == [
+        [4, 5, 25, 30], [4, 5, 25, 16], [4, 5, 25, 25]]
+
+
+def test_attention_keys(ask):
+    """Against the definition: the keys of every row of a tile are within its
+    [lo, hi), which holds no chunk in front of the first of them."""
+    rng = np.random.default_rng(3)
+    cases = []
+    for _ in range(400):
+        fresh, first = int(rng.integers(1, 40)), int(rng.integers(-20, 500))
+        keys = int(rng.integers(0, max(1, first + fresh + 1)))
+        i0 = int(rng.integers(0, fresh))
+        cases.append((fresh, first, keys, i0, int(rng.integers(i0, fresh)), int(rng.choice([0, 1, 17, 64, 300])),
+                      int(rng.choice([256, 512]))))
+    for (fresh, first, keys, i0, i1, window, split), (lo, hi, parts) in zip(
+            cases, ask(["keys " + " ".join(map(str, c)) for c in cases])):
+        seen = [k for i in range(i0, i1 + 1) for k in range(max(0, first + i - window + 1 if window else 0),
+                                                            min(keys, first + i + 1))]
+        assert lo % 64 == 0 and lo >= 0 and hi <= keys
+        assert parts == max(1, -(-(hi - lo) // split))
+        if seen:
+            assert lo <= min(seen) < lo + 64 and hi == max(seen) + 1
+    big = 2**31 - 1
+    assert ask([f"keys 1 {big - 1} {big} 0 0 0 {1 << 30}", f"keys 1 {big - 1} {big} 0 0 {big} 256",
+                f"keys 3 -3 0 0 2 {big} 256"]) == [[0, big, 2], [0, big, 8388608], [0, 0, 1]]
+
+
+def test_attention_cut(ask):
+    """Every row has a tile and every key a part, whatever the sizes."""
+    cases = [(r, kv, g, m, c) for r in (1, 3, 64, 65535) for kv in (1, 8) for g in (1, 7, 71) for m in (1, 5, 2048)
+             for c in (0, 1, 255, 4097, 131072, 2**31 - 1)]
+    for (r, kv, g, m, c), (tiles, split, parts) in zip(cases, ask(["cut " + " ".join(map(str, x)) for x in cases])):
+        assert 16 * tiles >= m * g > 16 * (tiles - 1)
+        assert split % 256 == 0 and split >= 256 and parts >= 1 and parts * split >= c
+        assert (parts - 1) * split < max(c, 1)
