@@ -190,9 +190,10 @@ def _ptr(a):
 
 def _stream(stream):
     if stream is None:
+        # (what torch.cuda.current_stream() wraps, without making a Stream: 0.3 us a call for 3)
         import torch
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-    return ctypes.c_void_p(stream)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return stream
 
 
 def type_size(dtype, n):
@@ -312,7 +313,7 @@ def _act(t):
 def _on_gpu(name, t, dtype, device, shape=None):
     """A contiguous device tensor of this type (and shape); its pointer."""
     if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or \
-            (shape is not None and tuple(t.shape) != shape):
+            (shape is not None and t.shape != shape):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor" + (f" of shape {shape}" if shape is not None else "")
                          + f" on cuda:{device}: got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
@@ -325,6 +326,8 @@ def _rows(name, t, like, heads=None, dim=None):
     if t.dtype != like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name} must be {like.dtype} on {like.device}: got {t.dtype} on {t.device}")
     n, h, d = t.shape
+    if t.is_contiguous():
+        return t.data_ptr(), h * d
     st = t.stride()
     if st[2] != 1 or (st[1] != d and h > 1) or (n > 1 and st[0] < h * d):
         raise ValueError(f"{name}: heads and values must be contiguous, rows must not overlap (strides {st})")
@@ -468,7 +471,8 @@ class HipBackend:
         max_tokens = int(max_tokens)
         if max_tokens < 0:
             raise ValueError(f"max_tokens {max_tokens} is negative")
-        out = PagePlan(*(torch.empty(k, dtype=i32, device=cached.device) for k in (n + 1, n, max_tokens, max_tokens, 2)))
+        sizes = (n + 1, n, max_tokens, max_tokens, 2)
+        out = PagePlan(*torch.empty(sum(sizes), dtype=i32, device=cached.device).split(sizes))  # one allocation
         _check(lib().gq_page_plan(c, m, n, page_size, f, free_pages.shape[0], t, tables.shape[1], out.q_start.data_ptr(),
                                   out.ctx_lens.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(), max_tokens,
                                   out.counts.data_ptr(), _stream(stream)))
@@ -487,18 +491,22 @@ class HipBackend:
         n, nq, hd = q.shape
         made = []
         if q_out is None:
-            q_out = torch.empty((n, nq, hd), dtype=q.dtype, device=q.device)
+            q_out = q.new_empty((n, nq, hd))
             made.append(q_out)
-        qo, qos = _rows("q_out", q_out, q, nq, hd)
+            qo, qos = q_out.data_ptr(), nq * hd
+        else:
+            qo, qos = _rows("q_out", q_out, q, nq, hd)
         kp = ko = None
         ks = kos = nk = 0
         if k is not None:
             kp, ks = _rows("k", k, q, None, hd)
             nk = k.shape[1]
             if k_out is None:
-                k_out = torch.empty((n, nk, hd), dtype=q.dtype, device=q.device)
+                k_out = q.new_empty((n, nk, hd))
                 made.append(k_out)
-            ko, kos = _rows("k_out", k_out, q, nk, hd)
+                ko, kos = k_out.data_ptr(), nk * hd
+            else:
+                ko, kos = _rows("k_out", k_out, q, nk, hd)
             if k.shape[0] != n or k_out.shape[0] != n:
                 raise ValueError("q, k and k_out must have the same number of tokens")
         if q_out.shape[0] != n:
@@ -532,8 +540,8 @@ class HipBackend:
         c = _cache(cache, dev)
         n = slots.shape[0]
         sp = _on_gpu("slots", slots, torch.int32, dev, (n,))
-        k, v = (torch.empty((n, c.n_kv_heads, c.head_dim), dtype=dtype or torch.float32, device=slots.device) for _ in "kv")
-        _check(lib().gq_kv8_read(ctypes.byref(c), sp, n, _act(k), _ptr(k), _ptr(v), _stream(stream)))
+        k, v = (slots.new_empty((n, c.n_kv_heads, c.head_dim), dtype=dtype or torch.float32) for _ in "kv")
+        _check(lib().gq_kv8_read(ctypes.byref(c), sp, n, _act(k), k.data_ptr(), v.data_ptr(), _stream(stream)))
         _kept(stream, k, v)
         return k, v
 
@@ -558,17 +566,22 @@ class HipBackend:
             raise ValueError(f"q is on {q.device}, the current device is cuda:{dev}")
         L, cr, made = lib(), ctypes.byref(c), []
         if out is None:
-            out = torch.empty((n, nh, hd), dtype=q.dtype, device=q.device)
+            out = q.new_empty((n, nh, hd))
             made.append(out)
-        op, os_ = _rows("out", out, q, nh, hd)
-        if out.shape[0] != n:
-            raise ValueError("q and out must have the same number of tokens")
-        if workspace is None:
-            need = L.gq_attn_kv8_workspace(cr, nh, n, nr, max_new, max_ctx)
-            if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            op, os_ = out.data_ptr(), nh * hd
+        else:
+            op, os_ = _rows("out", out, q, nh, hd)
+            if out.shape[0] != n:
+                raise ValueError("q and out must have the same number of tokens")
+        wp, wb = None, 0
+        if workspace is not None:
+            wp, wb = _on_gpu("workspace", workspace, torch.uint8, dev), workspace.numel()
+        else:
+            wb = L.gq_attn_kv8_workspace(cr, nh, n, nr, max_new, max_ctx)
+            if wb:
+                workspace = q.new_empty(wb, dtype=torch.uint8)
                 made.append(workspace)
-        wp, wb = (None, 0) if workspace is None else (_on_gpu("workspace", workspace, torch.uint8, dev), workspace.numel())
+                wp = workspace.data_ptr()
         _check(L.gq_attn_kv8(cr, dt, qp, qs, nh, n, tp, tables.shape[1], sp, cp, nr, max_new, max_ctx,
                              hd ** -0.5 if scale is None else scale, window, op, os_, wp, wb, _stream(stream)))
         _kept(stream, *made)
