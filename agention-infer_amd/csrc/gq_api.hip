@@ -1230,9 +1230,10 @@ int check_attn(const gq_kv8 *c, int n_heads, int n_tokens, int n_requests, int m
   if (int rc = check_kv8(c)) return rc;
   if (n_heads < 1 || n_heads % c->n_kv_heads)
     return fail(GQ_EINVAL, "gq_attn_kv8: %d heads are no multiple of %d KV heads", n_heads, c->n_kv_heads);
-  if (n_tokens < 0 || n_requests < 0 || n_requests > 65535 || max_new < 0 || max_ctx < 0)
-    return fail(GQ_EINVAL, "gq_attn_kv8: %d tokens, %d requests (at most 65535), max_new %d, max_ctx %d", n_tokens, n_requests,
-                max_new, max_ctx);
+  if (n_tokens < 0 || n_requests < 0 || n_requests > 65535 || max_new < 0 || max_ctx < 0 ||
+      max_ctx > 1 << 30)
+    return fail(GQ_EINVAL, "gq_attn_kv8: %d tokens, %d requests (at most 65535), max_new %d, max_ctx %d (at most 2^30)", n_tokens,
+                n_requests, max_new, max_ctx);
   if ((int64_t)max_new * (n_heads / c->n_kv_heads) > INT_MAX - 64)
     return fail(GQ_EINVAL, "gq_attn_kv8: max_new %d of %d heads: too many rows", max_new, n_heads);
   return GQ_OK;
@@ -1242,8 +1243,8 @@ int check_attn(const gq_kv8 *c, int n_heads, int n_tokens, int n_requests, int m
 extern "C" {
 size_t gq_attn_kv8_workspace(const gq_kv8 *c, int n_heads, int n_tokens, int n_requests, int max_new, int max_ctx) {
   if (check_attn(c, n_heads, n_tokens, n_requests, max_new, max_ctx)) return 0;
-  const gq::AttnCut cut = gq::attn_cut(n_requests, c->n_kv_heads, n_heads / c->n_kv_heads, max_new, max_ctx);
-  return gq::attn_kv8_bytes(n_tokens, n_heads, c->head_dim, cut.parts);
+  return gq::attn_kv8_bytes(n_tokens, n_heads, c->head_dim,
+                            gq::attn_cut(n_tokens, n_requests, c->n_kv_heads, n_heads / c->n_kv_heads, max_new, max_ctx));
 }
 
 int gq_attn_kv8(const gq_kv8 *c, int dtype, const void *q_dev, int64_t q_stride, int n_heads, int n_tokens,
@@ -1260,18 +1261,20 @@ int gq_attn_kv8(const gq_kv8 *c, int dtype, const void *q_dev, int64_t q_stride,
   if (int rc = check_rows("out", out_dev, out_stride, w, dtype)) return rc;
   if ((max_pages && !tables_dev) || !q_start_dev || !ctx_lens_dev) return fail(GQ_EINVAL, "gq_attn_kv8: null buffer");
   const int group = n_heads / c->n_kv_heads;
-  const gq::AttnCut cut = gq::attn_cut(n_requests, c->n_kv_heads, group, max_new, max_ctx);
-  const size_t need = gq::attn_kv8_bytes(n_tokens, n_heads, c->head_dim, cut.parts);
+  const gq::AttnCut cut = gq::attn_cut(n_tokens, n_requests, c->n_kv_heads, group, max_new, max_ctx);
+  const size_t need = gq::attn_kv8_bytes(n_tokens, n_heads, c->head_dim, cut);
   if (need && (!workspace_dev || workspace_bytes < need))
     return fail(GQ_ESHORT, "gq_attn_kv8: workspace: need %zu bytes, have %zu", need, workspace_dev ? workspace_bytes : 0);
   if (!aligned16(workspace_dev)) return fail(GQ_EINVAL, "gq_attn_kv8: the workspace must start at a multiple of 16 bytes");
-  if ((int64_t)cut.tiles * cut.parts > INT_MAX) return fail(GQ_EINVAL, "gq_attn_kv8: too many rows by keys in one call");
+  if (cut.rtiles * cut.rparts > INT_MAX || cut.ttiles * cut.tparts > INT_MAX / c->n_kv_heads)
+    return fail(GQ_EINVAL, "gq_attn_kv8: too many rows by keys in one call");
   if (int rc = ensure_init()) return rc;
   const gq::AttnArgs a{c->k,       c->v,         c->k_scale,    c->v_scale,    q_dev,      out_dev,        q_stride, out_stride,
                        tables_dev, q_start_dev,  ctx_lens_dev,  (float *)workspace_dev, scale, c->n_pages, c->page_size,
                        c->n_kv_heads, group,     n_tokens,      n_requests,    max_pages,  window,         max_new,  max_ctx,
-                       cut.split,  cut.parts};
-  return launched("attention", gq::launch_attn_kv8(a, dtype, c->head_dim, cut.tiles, (hipStream_t)stream));
+                       cut.split,  cut.rparts,   cut.tsplit,    cut.tparts,    cut.parts,
+                       c->page_size == 16 ? 0u : (uint32_t)(((1ull << 32) + c->page_size / 16 - 1) / (c->page_size / 16))};
+  return launched("attention", gq::launch_attn_kv8(a, dtype, c->head_dim, cut, (hipStream_t)stream));
 }
 
 int gq_sync(void *stream) {

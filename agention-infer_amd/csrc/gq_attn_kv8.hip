@@ -71,9 +71,11 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
   __shared__ float sm[NW][16], sl[NW][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const int tile = blockIdx.x / a.parts, part = blockIdx.x % a.parts, kh = blockIdx.y, b = blockIdx.z;
+  const int tile = blockIdx.x / a.rparts, part = blockIdx.x % a.rparts, kh = blockIdx.y, b = blockIdx.z;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
-  const int rows = min((int64_t)rq.fresh * a.group - (int64_t)tile * 16, (int64_t)16);
+  const int64_t all = (int64_t)rq.fresh * a.group;
+  if (a.tparts && all > ATTN_FEW_ROWS) return;  // k_attn_kv8_tiles has them
+  const int rows = min(all - (int64_t)tile * 16, (int64_t)16);
   if (rows <= 0) return;
   const int row0 = tile * 16;
   const AttnKeys ak = attn_keys(rq, row0 / a.group, (row0 + rows - 1) / a.group, a.window);
@@ -257,6 +259,265 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
   for (int e = 0; e < DPL; e++) op[e] = (T)(lr == 0.f ? 0.f : o[e] / lr);
 }
 
+// ------------------------------------------------------------ long tiles
+// A block is 256 query rows of a (request, KV head) over one part of its keys:
+// 8 waves of 32 rows that share chunks of 64 keys in LDS, as f16, two buffers,
+// one barrier a chunk; the codes of the next chunk are on their way in
+// registers meanwhile.  On v_mfma_f32_32x32x16_f16, transposed as above:
+//   S^T  lane (r = lane % 32, u = lane / 32): keys 8 (i / 4) + 4 u + i % 4 of each
+//        32, of row r.  A row's softmax is its lane's 32 values and one swap.
+//   O^T  depth step s takes the lane's values 8 s' .. 8 s' + 7, that is keys
+//        16 s + 4 u + {0..3} and 16 s + 8 + 4 u + {0..3}.
+// Both operands lie in LDS in the order in which lanes read them, 16 bytes a
+// lane.  K: step ks (dims 16 ks ..) of key tile kt, lane l at slot
+// (kt KS + ks) 64 + (l ^ 2 ks): the swap spreads the writes of a key's row over the
+// banks.  V: step s, tile e, lane l at slot (s DT + e) 64 + l holds the 8 keys
+// above of dim DT r + e; the thread that loads DT neighbouring bytes of those
+// 8 rows writes one slot of each tile.
+// The largest score may run ahead of M by 1.9 before O and l are scaled again, so
+// weights stay under 2^15.9, inside f16.
+constexpr int TILE_ROWS = ATTN_TILE_ROWS, TILE_THREADS = 512;
+typedef float a8_f32x16 __attribute__((ext_vector_type(16)));
+
+template <class T, int HD>
+__global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) {
+  constexpr bool SPLIT = std::is_same<T, float>::value;
+  constexpr int KS = HD / 16, DT = HD / 32, CPK = HD / 16, KL = 64 * CPK / 256;
+  constexpr float SHIFT = 14.f, AHEAD = 1.9f;
+  static_assert(DT == 2 || DT == 4, "head_dim 64 or 128");
+  __shared__ __align__(16) uint4 kl[2][2 * KS * 64], vl[2][4 * DT * 64];
+  __shared__ float4 scl[2][4];  // of 16 keys: ks, log2 vs, 1 / vs
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, u = lane >> 5;
+  // heads fastest: the blocks of one KV head's rows go to the same XCDs
+  const int kh = blockIdx.x % a.n_kv, bx = blockIdx.x / a.n_kv, b = blockIdx.y;
+  const int tile = bx / a.tparts, part = bx % a.tparts;
+  const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
+  const int64_t all = (int64_t)rq.fresh * a.group;
+  if (all <= ATTN_FEW_ROWS || (int64_t)tile * TILE_ROWS >= all) return;
+  const int row0 = tile * TILE_ROWS, rows = (int)min(all - row0, (int64_t)TILE_ROWS);
+  const AttnKeys ak = attn_keys(rq, row0 / a.group, (row0 + rows - 1) / a.group, a.window);
+  const int nparts = attn_parts(ak, a.tsplit);
+  if (part >= nparts) return;
+  const int klo = ak.lo + part * a.tsplit, khi = (int)min((int64_t)ak.hi, (int64_t)klo + a.tsplit);
+  const int nh = a.n_kv * a.group;
+
+  const int myrow = row0 + min(32 * wave + r, rows - 1), mytok = myrow / a.group, myhead = kh * a.group + myrow % a.group;
+  const bool mine = 32 * wave + r < rows;
+  const T *qp = (const T *)a.q + (int64_t)(rq.start + mytok) * a.q_stride + (int64_t)myhead * HD + 8 * u;
+  a8_f16x8 qh[KS], ql[SPLIT ? KS : 1];
+  float qf;
+  {
+    float qv[KS][8], qm = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        qv[ks][j] = (float)qp[16 * ks + j];
+        qm = fmaxf(qm, fabsf(qv[ks][j]));
+      }
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(qm), __float_as_uint(qm), false, false);
+    qm = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    int ex = 0;
+    (void)frexpf(qm, &ex);
+    const float up = qm > 0.f ? ldexpf(1.f, min(15 - ex, 126)) : 1.f;
+    qf = a.scale * 1.4426950408889634f / up;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float x = qv[ks][j] * up;
+        qh[ks][j] = (_Float16)x;
+        if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
+      }
+  }
+  const int see_hi = mine ? rq.first + mytok : -1;
+  const int64_t see_lo = a.window ? (int64_t)see_hi - a.window : -1;
+  // what the wave's rows see together (all: every row sees it)
+  const int w0 = row0 + min(32 * wave, rows - 1), w1 = row0 + min(32 * wave + 31, rows - 1);
+  const int any_hi = 32 * wave < rows ? rq.first + w1 / a.group : -1, all_hi = rq.first + w0 / a.group;
+  const int64_t any_lo = a.window ? (int64_t)all_hi - a.window : -1, all_lo = a.window ? (int64_t)any_hi - a.window : -1;
+  const bool full = 32 * wave + 31 < rows;
+
+  // staging: waves 0..3 take K (KL vectors each), 4..7 V (8 rows of 4 bytes)
+  const int *table = a.tables + (int64_t)b * a.wide;
+  const bool isv = tid >= 256;
+  const int t = tid & 255;
+  const int vset = t / (HD / 4), vq = t % (HD / 4), vs16 = vset >> 1, vu = vset & 1;
+  const bool vwork = isv && vset < 8, swork = vwork && vq == 0 && vu == 0;
+  auto block_of = [&](int k0, int j) { return (k0 >> 4) + (isv ? vs16 : (t + 256 * j) / CPK / 16); };
+  auto page_id = [&](int blk) {  // -1: no page, or no key of the part
+    if (16 * blk >= khi) return -1;
+    const int id = table[(int)a.div_page(blk)];
+    return id >= 0 && id < a.n_pages ? id : -1;
+  };
+  int ids[KL], now[KL];
+  uint4 raw[2];
+  float s_k = 0.f, s_v = 0.f;
+  auto load = [&](int k0) {  // codes of the chunk at k0, from pages `now`
+    if (!isv) {
+#pragma unroll
+      for (int j = 0; j < KL; j++) {
+        const int v = t + 256 * j, blk = block_of(k0, j), pj = a.div_page(blk);
+        const int64_t ph = (int64_t)max(now[j], 0) * a.n_kv + kh;
+        const int off = 16 * (blk - pj * (a.page >> 4)) + (v / CPK & 15);
+        raw[j] = *(const uint4 *)(a.kc + (ph * a.page + off) * HD + 16 * (v % CPK));
+      }
+    } else if (vwork) {
+      const int blk = block_of(k0, 0), pj = a.div_page(blk);
+      const int64_t ph = (int64_t)max(now[0], 0) * a.n_kv + kh;
+      const int8_t *p = a.vc + (ph * a.page + 16 * (blk - pj * (a.page >> 4)) + 4 * vu) * HD + 4 * vq;
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) w[j] = *(const uint32_t *)(p + (j < 4 ? j : j + 4) * HD);
+      raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      if (swork) {
+        s_k = a.ks[ph];
+        s_v = a.vs[ph];
+      }
+    }
+  };
+  auto store = [&](int buf) {
+    if (!isv) {
+#pragma unroll
+      for (int j = 0; j < KL; j++) {
+        const int v = t + 256 * j, key = v / CPK, c = v % CPK;
+        uint4 lo, hi;
+        f16_of_dword(raw[j].x, lo.x, lo.y);
+        f16_of_dword(raw[j].y, lo.z, lo.w);
+        f16_of_dword(raw[j].z, hi.x, hi.y);
+        f16_of_dword(raw[j].w, hi.z, hi.w);
+        uint4 *p = kl[buf] + ((key >> 5) * KS + c) * 64;
+        p[(key & 31) ^ (2 * c & 15)] = lo;
+        p[32 + ((key & 31) ^ (2 * c & 15))] = hi;
+      }
+    } else if (vwork) {
+      const uint32_t w[8] = {raw[0].x ^ 0x80808080u, raw[0].y ^ 0x80808080u, raw[0].z ^ 0x80808080u, raw[0].w ^ 0x80808080u,
+                             raw[1].x ^ 0x80808080u, raw[1].y ^ 0x80808080u, raw[1].z ^ 0x80808080u, raw[1].w ^ 0x80808080u};
+      // byte e of the 8 rows is dim 4 vq + e: row (4 vq + e) / DT of tile (4 vq + e) % DT
+      auto put = [&](int e, uint4 f) {
+        const int d = 4 * vq + e;
+        vl[buf][(vs16 * DT + d % DT) * 64 + 32 * vu + d / DT] = f;
+      };
+      put(0, make_uint4(f16_of_bytes<0>(w[0], w[1]), f16_of_bytes<0>(w[2], w[3]), f16_of_bytes<0>(w[4], w[5]), f16_of_bytes<0>(w[6], w[7])));
+      put(1, make_uint4(f16_of_bytes<1>(w[0], w[1]), f16_of_bytes<1>(w[2], w[3]), f16_of_bytes<1>(w[4], w[5]), f16_of_bytes<1>(w[6], w[7])));
+      put(2, make_uint4(f16_of_bytes<2>(w[0], w[1]), f16_of_bytes<2>(w[2], w[3]), f16_of_bytes<2>(w[4], w[5]), f16_of_bytes<2>(w[6], w[7])));
+      put(3, make_uint4(f16_of_bytes<3>(w[0], w[1]), f16_of_bytes<3>(w[2], w[3]), f16_of_bytes<3>(w[4], w[5]), f16_of_bytes<3>(w[6], w[7])));
+      if (swork) scl[buf][vs16] = now[0] < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(s_k, log2f(s_v), 1.f / s_v, 0.f);
+    }
+  };
+
+  float M = -INFINITY, l = 0.f;
+  a8_f32x16 O[DT];
+#pragma unroll
+  for (int e = 0; e < DT; e++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) O[e][i] = 0.f;
+
+#pragma unroll
+  for (int j = 0; j < KL; j++) now[j] = page_id(block_of(klo, j));
+  if (klo < khi) load(klo);
+#pragma unroll
+  for (int j = 0; j < KL; j++) ids[j] = page_id(block_of(klo + 64, j));
+  int buf = 0;
+  for (int k0 = klo; k0 < khi; k0 += 64, buf ^= 1) {
+    store(buf);
+    if (k0 + 64 < khi) {
+#pragma unroll
+      for (int j = 0; j < KL; j++) now[j] = ids[j];
+      load(k0 + 64);
+#pragma unroll
+      for (int j = 0; j < KL; j++) ids[j] = page_id(block_of(k0 + 128, j));
+    }
+    __syncthreads();
+    if (k0 > any_hi || k0 + 63 <= any_lo) continue;
+    a8_f32x16 z[2];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) z[kt][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const a8_f16x8 k8 = __builtin_bit_cast(a8_f16x8, kl[buf][(kt * KS + ks) * 64 + (lane ^ (2 * ks & 15))]);
+        z[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[ks], z[kt], 0, 0, 0);
+        if (SPLIT) z[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[ks], z[kt], 0, 0, 0);
+      }
+    }
+    float ivs[4];
+    const bool seen = full && k0 + 63 <= all_hi && k0 > all_lo;  // by every row
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const float4 sc = scl[buf][q];
+      const float f = sc.x * qf;
+      ivs[q] = sc.z;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float x = fmaf(z[q >> 1][8 * (q & 1) + i], f, sc.y);
+        if (!seen) {
+          const int64_t key = k0 + 16 * q + 8 * (i >> 2) + 4 * u + (i & 3);
+          if (!(key <= see_hi && key > see_lo && sc.y != -INFINITY)) x = -INFINITY;
+        }
+        z[q >> 1][8 * (q & 1) + i] = x;
+        mx = fmaxf(mx, x);
+      }
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    const bool more = mx > M + AHEAD;
+    if (__any(more)) {
+      const float Mn = more ? mx : M, alpha = !more ? 1.f : M == -INFINITY ? 0.f : exp2_raw(M - Mn);
+      M = Mn;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < DT; e++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) O[e][i] *= alpha;
+    }
+    const float base = M == -INFINITY ? 0.f : M - SHIFT;
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      a8_f16x8 ph8, pl8;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float p = exp2_raw(z[s >> 1][8 * (s & 1) + j] - base);
+        // (a key that is not seen adds nothing, whatever its page's scale)
+        l = fmaf(p, !seen && p == 0.f ? 0.f : ivs[s], l);
+        ph8[j] = (_Float16)p;
+        if (SPLIT) pl8[j] = (_Float16)(p - (float)ph8[j]);
+      }
+#pragma unroll
+      for (int e = 0; e < DT; e++) {
+        const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, vl[buf][(s * DT + e) * 64 + lane]);
+        O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph8, O[e], 0, 0, 0);
+        if (SPLIT) O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl8, O[e], 0, 0, 0);
+      }
+    }
+  }
+  {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  if (!mine) return;
+  // row r's dims DT (8 (i / 4) + 4 u + i % 4) + e
+  if (nparts > 1) {
+    float *p = a.part + (((int64_t)(rq.start + mytok) * nh + myhead) * a.parts + part) * (HD + 4);
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+#pragma unroll
+      for (int e = 0; e < DT; e += 2)
+        *(float2 *)(p + DT * (8 * (i / 4) + 4 * u + i % 4) + e) = make_float2(O[e][i], O[e + 1][i]);
+    if (u == 0) *(float2 *)(p + HD) = make_float2(M, l);
+    return;
+  }
+  T *op = (T *)a.out + (int64_t)(rq.start + mytok) * a.out_stride + (int64_t)myhead * HD;
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+#pragma unroll
+    for (int e = 0; e < DT; e++) op[DT * (8 * (i / 4) + 4 * u + i % 4) + e] = (T)(l == 0.f ? 0.f : O[e][i] / l);
+}
+
 // The parts of a row joined: o = sum_p O_p 2^(M_p - M) / sum_p l_p 2^(M_p - M).
 // A wave is one row; rows of one part are written already.
 constexpr int JOIN_THREADS = 256;
@@ -268,9 +529,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
   const int64_t row = (int64_t)blockIdx.x * (JOIN_THREADS / 64) + (threadIdx.x >> 6);
   const int64_t all = (int64_t)rq.fresh * a.group;
   if (row >= all) return;
-  const int row0 = (int)(row / 16 * 16);  // of its tile
-  const AttnKeys ak = attn_keys(rq, row0 / a.group, (int)(min((int64_t)row0 + 16, all) - 1) / a.group, a.window);
-  const int n = attn_parts(ak, a.split);
+  const bool tiles = a.tparts && all > ATTN_FEW_ROWS;
+  const int height = tiles ? TILE_ROWS : 16, row0 = (int)(row / height * height);  // of its tile
+  const AttnKeys ak = attn_keys(rq, row0 / a.group, (int)((min((int64_t)row0 + height, all) - 1) / a.group), a.window);
+  const int n = attn_parts(ak, tiles ? a.tsplit : a.split);
   if (n == 1) return;
   const int nh = a.n_kv * a.group, tok = rq.start + (int)(row / a.group), head = kh * a.group + (int)(row % a.group);
   const float *p = a.part + ((int64_t)tok * nh + head) * a.parts * LD;
@@ -290,27 +552,32 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
   for (int e = 0; e < DPL; e++) op[e] = (T)(l == 0.f ? 0.f : o[e] / l);
 }
 
-size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, int parts) {
-  return parts > 1 ? (size_t)n_tokens * n_heads * parts * (hd + 4) * sizeof(float) : 0;
+size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, const AttnCut &c) {
+  return c.parts > 1 ? (size_t)n_tokens * n_heads * c.parts * (hd + 4) * sizeof(float) : 0;
 }
 
 template <class T, int HD>
-static void attn_launch(const AttnArgs &a, int tiles, hipStream_t st) {
-  hipLaunchKernelGGL((k_attn_kv8_rows<T, HD>), dim3(tiles * a.parts, a.n_kv, a.n_requests), dim3(ROWS_THREADS), 0, st, a);
-  if (a.parts > 1) {
+static void attn_launch(const AttnArgs &a, const AttnCut &c, hipStream_t st) {
+  if (c.tparts)
+    hipLaunchKernelGGL((k_attn_kv8_tiles<T, HD>), dim3((unsigned)(c.ttiles * c.tparts * a.n_kv), a.n_requests),
+                       dim3(TILE_THREADS), 0, st, a);
+  if (c.rtiles)
+    hipLaunchKernelGGL((k_attn_kv8_rows<T, HD>), dim3((unsigned)(c.rtiles * c.rparts), a.n_kv, a.n_requests),
+                       dim3(ROWS_THREADS), 0, st, a);
+  if (c.parts > 1) {
     const int64_t rows = (int64_t)a.max_new * a.group;
     hipLaunchKernelGGL((k_attn_kv8_join<T, HD>), dim3((unsigned)((rows + 3) / 4), a.n_kv, a.n_requests), dim3(JOIN_THREADS), 0,
                        st, a);
   }
 }
 
-hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, int tiles, hipStream_t st) {
+hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, const AttnCut &c, hipStream_t st) {
   auto go = [&](auto zero) {
     typedef decltype(zero) T;
     if (hd == 64)
-      attn_launch<T, 64>(a, tiles, st);
+      attn_launch<T, 64>(a, c, st);
     else
-      attn_launch<T, 128>(a, tiles, st);
+      attn_launch<T, 128>(a, c, st);
   };
   if (dtype == T_F32)
     go(0.f);

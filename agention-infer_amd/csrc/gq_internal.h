@@ -6,6 +6,7 @@
 
 #include "gq_gemm_plan.h"
 #include "gq_layout.h"
+#include "gq_paged.h"
 
 // The public handle (opaque in gq.h).
 struct gq_weight {
@@ -340,9 +341,13 @@ struct AttnArgs {
   float *part;  // [n_tokens][n_heads][parts][hd + 4]: O, then m, l
   float scale;
   int n_pages, page, n_kv, group, n_tokens, n_requests, wide, window;
-  int max_new, max_ctx, split, parts;
+  int max_new, max_ctx;
+  int split, rparts, tsplit, tparts, parts;  // AttnCut
+  uint32_t page_magic;  // 2^32 / (page / 16) rounded up, 0 for 1
+  // page of 16-key block n < 2^27 (n (d - 1) < 2^32, so the product's floor is exact)
+  __device__ __forceinline__ int div_page(int n) const { return page_magic ? (int)__umulhi((uint32_t)n, page_magic) : n; }
 };
-size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, int parts);
-hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, int tiles, hipStream_t st);
+size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, const AttnCut &c);
+hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, const AttnCut &c, hipStream_t st);
 
 }  // namespace gq

@@ -371,7 +371,7 @@ int gq_kv8_read(const gq_kv8 *cache, const int *slots_dev, int n, int dtype, voi
  * max_new and max_ctx bound the rows and positions of a request: rows past
  * max_new are not computed, keys past max_ctx (or the table) not seen.  Rows
  * that belong to no request, behind q_start[n_requests] among them, are left
- * as they are.  At most 65535 requests; a new row's own k and v are in the
+ * as they are.  At most 65535 requests, max_ctx at most 2^30; a new row's own k and v are in the
  * cache before the call.  Buffers and strides are multiples of 16 bytes; out
  * overlaps nothing.
  * The workspace is the caller's: gq_attn_kv8_workspace bytes (0 where none is

@@ -5,7 +5,8 @@
 //   owner N V AT0 .. ATN  ->  owner_of
 //   req S E CTX N WIDE PAGE MAXCTX  ->  start fresh first keys of attn_request
 //   keys FRESH FIRST KEYS I0 I1 WINDOW SPLIT  ->  lo hi of attn_keys, attn_parts
-//   cut REQUESTS KV GROUP MAXNEW MAXCTX  ->  tiles split parts of attn_cut
+//   cut TOKENS REQUESTS KV GROUP MAXNEW MAXCTX  ->  rtiles split rparts ttiles tsplit
+//                                               tparts parts of attn_cut
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -39,10 +40,11 @@ int main() {
       const gq::AttnKeys k = gq::attn_keys(r, i0, i1, window);
       std::printf("%d %d %d\n", k.lo, k.hi, gq::attn_parts(k, split));
     } else if (!std::strcmp(what, "cut")) {
-      int nr, kv, group, fresh, ctx;
-      if (std::scanf("%d %d %d %d %d", &nr, &kv, &group, &fresh, &ctx) != 5) return 1;
-      const gq::AttnCut t = gq::attn_cut(nr, kv, group, fresh, ctx);
-      std::printf("%d %d %d\n", t.tiles, t.split, t.parts);
+      int n, nr, kv, group, fresh, ctx;
+      if (std::scanf("%d %d %d %d %d %d", &n, &nr, &kv, &group, &fresh, &ctx) != 6) return 1;
+      const gq::AttnCut t = gq::attn_cut(n, nr, kv, group, fresh, ctx);
+      std::printf("%lld %d %d %lld %d %d %d\n", (long long)t.rtiles, t.split, t.rparts, (long long)t.ttiles, t.tsplit,
+                  t.tparts, t.parts);
     } else {
       return 1;
     }

@@ -88,7 +88,8 @@ ATTN = dict(dtype=gq.F32, q=P, qs=256, nh=4, n=8, tables=P, wide=4, q_start=P, c
 @pytest.mark.parametrize("change,code,text", [
     (dict(dtype=12), EDTYPE, "Q4_K"), (dict(nh=3), EINVAL, "3 heads"), (dict(nh=0), EINVAL, "0 heads"),
     (dict(n=-1), EINVAL, "-1 tokens"), (dict(nr=-1), EINVAL, "-1 requests"), (dict(nr=65536), EINVAL, "at most 65535"),
-    (dict(max_new=-1), EINVAL, "max_new -1"), (dict(max_ctx=-1), EINVAL, "max_ctx -1"), (dict(wide=-1), EINVAL, "max_pages -1"),
+    (dict(max_new=-1), EINVAL, "max_new -1"), (dict(max_ctx=-1), EINVAL, "max_ctx -1"),
+    (dict(max_ctx=2**30 + 1), EINVAL, "at most 2"), (dict(wide=-1), EINVAL, "max_pages -1"),
     (dict(window=-1), EINVAL, "window -1"), (dict(scale=math.inf), EINVAL, "scale"), (dict(scale=math.nan), EINVAL, "scale"),
     (dict(max_new=2**30), EINVAL, "too many rows"), (dict(qs=255), EINVAL, "q: rows"), (dict(os=128), EINVAL, "out: rows"),
     (dict(qs=257), EINVAL, "multiples of 16"), (dict(os=258), EINVAL, "multiples of 16"), (dict(q=P + 4), EINVAL, "multiples of 16"),
@@ -260,9 +261,16 @@ def test_attention_keys(ask):
 
 def test_attention_cut(ask):
     """Every row has a tile and every key a part, whatever the sizes."""
-    cases = [(r, kv, g, m, c) for r in (1, 3, 64, 65535) for kv in (1, 8) for g in (1, 7, 71) for m in (1, 5, 2048)
-             for c in (0, 1, 255, 4097, 131072, 2**31 - 1)]
-    for (r, kv, g, m, c), (tiles, split, parts) in zip(cases, ask(["cut " + " ".join(map(str, x)) for x in cases])):
-        assert 16 * tiles >= m * g > 16 * (tiles - 1)
-        assert split % 256 == 0 and split >= 256 and parts >= 1 and parts * split >= c
-        assert (parts - 1) * split < max(c, 1)
+    cases = [(n, r, kv, g, m, c) for n in (1, 700, 2**31 - 1) for r in (1, 3, 64, 65535) for kv in (1, 8) for g in (1, 7, 71)
+             for m in (1, 5, 2048) for c in (0, 1, 255, 4097, 131072, 2**31 - 1)]
+    for (n, r, kv, g, m, c), (rtiles, split, rparts, ttiles, tsplit, tparts, parts) in zip(
+            cases, ask(["cut " + " ".join(map(str, x)) for x in cases])):
+        few = min(m * g, 64)
+        assert 16 * rtiles >= few > 16 * (rtiles - 1)
+        assert split % 64 == 0 and split > 0 and rparts >= 1 and rparts * split >= c and (rparts - 1) * split < max(c, 1)
+        if m * g > 64:
+            assert 256 * ttiles >= m * g > 256 * (ttiles - 1)
+            assert tsplit % 64 == 0 and tsplit > 0 and tparts * tsplit >= c and (tparts - 1) * tsplit < max(c, 1)
+        else:
+            assert ttiles == tparts == 0
+        assert parts == max(rparts, tparts)
