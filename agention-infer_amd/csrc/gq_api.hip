@@ -1266,13 +1266,14 @@ int gq_attn_kv8(const gq_kv8 *c, int dtype, const void *q_dev, int64_t q_stride,
   if (need && (!workspace_dev || workspace_bytes < need))
     return fail(GQ_ESHORT, "gq_attn_kv8: workspace: need %zu bytes, have %zu", need, workspace_dev ? workspace_bytes : 0);
   if (!aligned16(workspace_dev)) return fail(GQ_EINVAL, "gq_attn_kv8: the workspace must start at a multiple of 16 bytes");
-  if (cut.rtiles * cut.rparts > INT_MAX || cut.ttiles * cut.tparts > INT_MAX / c->n_kv_heads)
+  const int64_t of = (int64_t)c->n_kv_heads * n_requests;  // (a grid's blocks)
+  if (cut.rtiles * cut.rparts > INT_MAX / of || cut.ttiles * cut.tparts > INT_MAX / of)
     return fail(GQ_EINVAL, "gq_attn_kv8: too many rows by keys in one call");
   if (int rc = ensure_init()) return rc;
   const gq::AttnArgs a{c->k,       c->v,         c->k_scale,    c->v_scale,    q_dev,      out_dev,        q_stride, out_stride,
                        tables_dev, q_start_dev,  ctx_lens_dev,  (float *)workspace_dev, scale, c->n_pages, c->page_size,
                        c->n_kv_heads, group,     n_tokens,      n_requests,    max_pages,  window,         max_new,  max_ctx,
-                       cut.split,  cut.rparts,   cut.tsplit,    cut.tparts,    cut.parts,
+                       (int)cut.rtiles, (int)cut.ttiles, cut.few, cut.split, cut.rparts,   cut.tsplit,    cut.tparts,    cut.parts,
                        c->page_size == 16 ? 0u : (uint32_t)(((1ull << 32) + c->page_size / 16 - 1) / (c->page_size / 16))};
   return launched("attention", gq::launch_attn_kv8(a, dtype, c->head_dim, cut, (hipStream_t)stream));
 }

@@ -6,15 +6,17 @@
 // with codes c, and one scale ks, vs for each page and KV head.  Scores are kept
 // in base 2 with the V scale in them, z_t = log2(e) s_t + log2 vs_t, so that
 // with M the largest z so far
-//   w_t = 2^(z_t - M + 15),  O = sum_t w_t c^V_t,  l = sum_t w_t / vs_t,  o = O / l
+//   w_t = 2^(z_t - M + 14),  O = sum_t w_t c^V_t,  l = sum_t w_t / vs_t,  o = O / l
 // takes the scale of each page for no more than an fma per score and one per
-// sum.  The 15 puts the weights into the upper range of f16, so that those down
-// to 2^-29 of the largest keep all of its bits.
+// sum.  The 14 puts the weights into the upper range of f16, so that those down
+// to 2^-28 of the largest keep all of its bits.  The largest z may run ahead of M
+// by 1.9 before O and l are scaled again: weights stay under 2^15.9, inside f16.
 //
 // Both products run on v_mfma_f32_16x16x32_f16: codes are exact in f16; q is
 // scaled by a power of two and split into f16 hi + lo, as are the weights, for
 // f32 activations (22 bits each), and rounded to one f16 for 16-bit ones (11
 // bits: their own rounding is as large).
+#include <algorithm>
 #include <type_traits>
 
 #include "gq_device.h"
@@ -26,6 +28,7 @@ namespace gq {
 typedef _Float16 a8_f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 a8_f16x2 __attribute__((ext_vector_type(2)));
 typedef float a8_f32x4 __attribute__((ext_vector_type(4)));
+constexpr float SHIFT = 14.f, AHEAD = 1.9f;
 
 // f16 of the two codes whose bytes (biased by 128) are bytes 0 and 2 of x:
 // 0x6400 | u is 1024 + u exactly.
@@ -45,54 +48,72 @@ __device__ __forceinline__ uint32_t f16_of_bytes(uint32_t a, uint32_t b) {
   return f16_of_biased(__builtin_amdgcn_perm(b, a, 0x0c040c00u + 0x00010001u * B) | 0x64006400u);
 }
 
+// (arguments far from denormal results and, for the scales, >= 2^-60)
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_raw(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float rcp_raw(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// What the instruction scheduler puts next (LDS reads, matrix instructions).
+template <int N>
+__device__ __forceinline__ void sched_ds() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
+template <int N>
+__device__ __forceinline__ void sched_mfma() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
+
+// The last position in front of what a row at `pos` sees.
+__device__ __forceinline__ int first_hidden(int pos, int window) {
+  return window && pos >= window ? pos - window : -1;
+}
 
 // ------------------------------------------------------------- row tiles
 // A block is one tile of 16 query rows of a (request, KV head) over one part
 // of its keys.  Rows are the request's tokens by the KV head's query heads, so
 // the heads that share K and V, and a draft's tokens, share one read of them.
-// Its 4 waves take chunks of 64 keys in turn, each with its own M, l, O, and
+// Its 4 waves take chunks of 32 keys in turn, each with its own M, l, O, and
 // meet once at the end; nothing goes through LDS before that:
 //   S^T = K . q^T  A = 16 keys x 32 dims.  Lane (m = lane % 16, g = lane / 16)
-//         takes row m's bytes [HD/4 g, HD/4 (g + 1)), so a key's row is read by
-//         4 lanes in 16-byte loads; step ks multiplies the 8 of them at 8 ks,
-//         and q's fragments hold the same dims.
+//         takes 16 bytes of row m at 64 i + 16 g (i < HD / 64), so a load reads
+//         whole runs of 64; step ks multiplies the 8 of them at 8 (ks % 2) of
+//         i = ks / 2, and q's fragments hold the same dims.
 //   O^T = V^T . P^T  B = the lane's own weights (keys 16 t0 + 4 g + j, j < 4,
 //         and 16 t1 + 4 g + j - 4), A = V^T in that key order: the lane loads
 //         HD/16 bytes at HD/16 m of these 8 rows, and byte e of the 8 is row m
 //         of tile e, so tile e of O^T holds dims HD/16 m + e.
 constexpr int ROWS_THREADS = 256;
 template <class T, int HD>
-__global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
+__global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
   constexpr bool SPLIT = std::is_same<T, float>::value;  // hi + lo operands
   constexpr int KS = HD / 32, KV = HD / 64, DPL = HD / 16;
-  constexpr int NW = ROWS_THREADS / 64, LD = HD + 4;
+  constexpr int NW = ROWS_THREADS / 64, LD = HD + 4, NT = 2, CHUNK = 16 * NT;
   __shared__ __align__(16) float so[NW][16][LD];
   __shared__ float sm[NW][16], sl[NW][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m = lane & 15, g = lane >> 4;
-  const int tile = blockIdx.x / a.rparts, part = blockIdx.x % a.rparts, kh = blockIdx.y, b = blockIdx.z;
+  // Blocks of one tile and part follow each other over heads and requests:
+  // neighbours go to the XCDs in turn, so that each gets its share of the long
+  // requests (parts in the grid's x, 8 of them: 64 requests of 128 .. 8192 keys
+  // in 156 us, the ones of part 7 all on one XCD).
+  const int of = a.n_kv * a.n_requests, i0 = blockIdx.x % of, step = blockIdx.x / of;
+  const int kh = i0 % a.n_kv, b = i0 / a.n_kv, tile = step % a.rtiles, part = step / a.rtiles;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
   const int64_t all = (int64_t)rq.fresh * a.group;
-  if (a.tparts && all > ATTN_FEW_ROWS) return;  // k_attn_kv8_tiles has them
+  if (a.tparts && all > a.few) return;  // k_attn_kv8_tiles has them
   const int rows = min(all - (int64_t)tile * 16, (int64_t)16);
   if (rows <= 0) return;
   const int row0 = tile * 16;
   const AttnKeys ak = attn_keys(rq, row0 / a.group, (row0 + rows - 1) / a.group, a.window);
   const int nparts = attn_parts(ak, a.split);
   if (part >= nparts) return;
-  const int64_t klo = (int64_t)ak.lo + (int64_t)part * a.split;
-  const int khi = (int)min((int64_t)ak.hi, klo + a.split);
+  const int klo = ak.lo + part * a.split, khi = (int)min((int64_t)ak.hi, (int64_t)klo + a.split);
   const int nh = a.n_kv * a.group;
 
   // q: row m's values of this lane's dims, scaled to 2^14 .. 2^15
   const int myrow = row0 + min(m, rows - 1), mytok = myrow / a.group, myhead = kh * a.group + myrow % a.group;
-  const T *qp = (const T *)a.q + (int64_t)(rq.start + mytok) * a.q_stride + (int64_t)myhead * HD + (HD / 4) * g;
+  const T *qp = (const T *)a.q + (int64_t)(rq.start + mytok) * a.q_stride + (int64_t)myhead * HD + 16 * g;
   float qv[HD / 4];
   float qm = 0.f;
 #pragma unroll
   for (int i = 0; i < HD / 4; i++) {
-    qv[i] = (float)qp[i];
+    qv[i] = (float)qp[64 * (i / 16) + i % 16];
     qm = fmaxf(qm, fabsf(qv[i]));
   }
   qm = lane_groups_max(qm);
@@ -109,9 +130,10 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
       qh[ks][j] = (_Float16)x;
       if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
     }
-  // keys that row m sees: (see_lo, see_hi]
+  // keys that row m sees: (see_lo, see_hi]; all_lo, all_hi: that each row sees
   const int see_hi = m < rows ? rq.first + mytok : -1;
-  const int64_t see_lo = a.window ? (int64_t)see_hi - a.window : -1;
+  const int see_lo = first_hidden(see_hi, a.window), all_hi = rows == 16 ? rq.first + row0 / a.group : -1;
+  const int all_lo = first_hidden(rq.first + (row0 + rows - 1) / a.group, a.window);
 
   float M = -INFINITY, l = 0.f;
   a8_f32x4 O[DPL];
@@ -119,42 +141,56 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
   for (int e = 0; e < DPL; e++) O[e] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
   const int *table = a.tables + (int64_t)b * a.wide;
 
-  for (int64_t k0 = klo + 64 * wave; k0 < khi; k0 += 64 * NW) {
-    uint4 kf[4][KV];
-    uint32_t vf[4][4][DPL / 4];
-    float ksc[4], vsc[4];
-    bool ok[4];
-    int pj = (int)(k0 / a.page), off = (int)(k0 % a.page);
+  // The chunk at k0: `ids` its pages, K, V and scales on their way while the
+  // chunk before is worked on (two sets of registers; chunks of 64 keys take
+  // 128 of them and spill).
+  struct Chunk {
+    uint4 kf[NT][KV];
+    uint32_t vf[NT][4][DPL / 4];
+    float ksc[NT], vsc[NT];
+    bool ok[NT];
+  };
+  auto pages = [&](int k0, int (&ids)[NT]) {
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      int id = k0 + 16 * t < khi ? table[pj] : -1;
-      ok[t] = id >= 0 && id < a.n_pages;
-      if (!ok[t]) id = 0;  // (its rows are read and not used)
-      const int64_t ph = (int64_t)id * a.n_kv + kh;
-      ksc[t] = a.ks[ph];
-      vsc[t] = a.vs[ph];
-      const int8_t *kp = a.kc + (ph * a.page + off + m) * HD + (HD / 4) * g;
-      const int8_t *vp = a.vc + (ph * a.page + off + 4 * g) * HD + DPL * m;
+    for (int t = 0; t < NT; t++) {
+      const int blk = (k0 >> 4) + t;
+      const int id = 16 * blk < khi ? table[a.div_page(blk)] : -1;
+      ids[t] = id < a.n_pages ? id : -1;
+    }
+  };
+  auto load = [&](int k0, const int (&ids)[NT], Chunk &c) {
+    const int p16 = a.page >> 4;
 #pragma unroll
-      for (int i = 0; i < KV; i++) kf[t][i] = *(const uint4 *)(kp + 16 * i);
+    for (int t = 0; t < NT; t++) {
+      const int blk = (k0 >> 4) + t, off = 16 * (blk - a.div_page(blk) * p16);
+      c.ok[t] = ids[t] >= 0;  // (else page 0's rows are read and not used)
+      const int64_t ph = (int64_t)max(ids[t], 0) * a.n_kv + kh;
+      c.ksc[t] = a.ks[ph];
+      c.vsc[t] = a.vs[ph];
+      const int8_t *kp = a.kc + (ph * a.page + off) * HD + (m * HD + 16 * g);
+      const int8_t *vp = a.vc + (ph * a.page + off) * HD + (4 * g * HD + DPL * m);
 #pragma unroll
-      for (int j = 0; j < 4; j++)
+      for (int i = 0; i < KV; i++) c.kf[t][i] = ldw4(kp + 64 * i);
 #pragma unroll
-        for (int i = 0; i < DPL / 4; i++) vf[t][j][i] = *(const uint32_t *)(vp + j * HD + 4 * i);
-      off += 16;
-      if (off == a.page) {
-        off = 0;
-        pj++;
+      for (int j = 0; j < 4; j++) {
+        if constexpr (DPL == 8) {
+          const uint2 w = ldw2(vp + j * HD);
+          c.vf[t][j][0] = w.x;
+          c.vf[t][j][1] = w.y;
+        } else {
+          c.vf[t][j][0] = ldw1(vp + j * HD);
+        }
       }
     }
-    float z[4][4], ivs[4];
-    float mx = -INFINITY;
+  };
+  auto work = [&](int k0, const Chunk &c) {
+    float z[NT][4], ivs[NT];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < NT; t++) {
       a8_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        const uint4 w = kf[t][ks / 2];
+        const uint4 w = c.kf[t][ks / 2];
         uint4 f;
         f16_of_dword(ks & 1 ? w.z : w.x, f.x, f.y);
         f16_of_dword(ks & 1 ? w.w : w.y, f.z, f.w);
@@ -162,22 +198,42 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[ks], acc, 0, 0, 0);
         if (SPLIT) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[ks], acc, 0, 0, 0);
       }
-      const float f = ksc[t] * qf, lv = log2f(vsc[t]);
-      ivs[t] = 1.f / vsc[t];
+      const float f = c.ksc[t] * qf, lv = log2_raw(c.vsc[t]);
+      ivs[t] = rcp_raw(c.vsc[t]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int64_t key = k0 + 16 * t + 4 * g + i;
-        const bool sees = ok[t] && key <= see_hi && key > see_lo;
-        z[t][i] = sees ? fmaf(acc[i], f, lv) : -INFINITY;
-        mx = fmaxf(mx, z[t][i]);
-      }
+      for (int i = 0; i < 4; i++) z[t][i] = fmaf(acc[i], f, lv);
     }
-    const float Mn = fmaxf(M, lane_groups_max(mx));
-    const float alpha = M == -INFINITY ? 0.f : exp2_raw(M - Mn), base = Mn == -INFINITY ? 0.f : Mn - 15.f;
-    M = Mn;
-    l *= alpha;
+    bool seen = k0 + CHUNK - 1 <= all_hi && k0 > all_lo;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int t = 0; t < NT; t++) seen = seen && c.ok[t];
+    if (!seen) {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int key = k0 + 16 * t + 4 * g + i;
+          if (!(c.ok[t] && key <= see_hi && key > see_lo)) z[t][i] = -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) mx = fmaxf(mx, z[t][i]);
+    mx = lane_groups_max(mx);
+    const bool more = mx > M + AHEAD;
+    if (__any(more)) {
+      const float Mn = more ? mx : M, alpha = !more ? 1.f : M == -INFINITY ? 0.f : exp2_raw(M - Mn);
+      M = Mn;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < DPL; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) O[e][i] *= alpha;
+    }
+    const float base = M == -INFINITY ? 0.f : M - SHIFT;
+#pragma unroll
+    for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float p = exp2_raw(z[t][i] - base);
@@ -186,11 +242,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
         l = fmaf(p, p == 0.f ? 0.f : ivs[t], l);
       }
 #pragma unroll
-    for (int e = 0; e < DPL; e++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) O[e][i] *= alpha;
-#pragma unroll
-    for (int st = 0; st < 2; st++) {
+    for (int st = 0; st < NT / 2; st++) {
       a8_f16x8 ph8, pl8;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -200,23 +252,57 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < DPL / 4; i++) {
-        uint32_t w[8];
+        // keys in pairs: bytes a0 b0 a1 b1 and a2 b2 a3 b3 of rows a, b
+        uint32_t lo[4], hi[4];
 #pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = vf[2 * st + j / 4][j & 3][i] ^ 0x80808080u;
-        auto step = [&](a8_f32x4 &o, uint4 f) {
-          const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, f);
+        for (int j = 0; j < 4; j++) {
+          const uint32_t x = c.vf[2 * st + j / 2][2 * (j & 1)][i] ^ 0x80808080u;
+          const uint32_t y = c.vf[2 * st + j / 2][2 * (j & 1) + 1][i] ^ 0x80808080u;
+          lo[j] = __builtin_amdgcn_perm(y, x, 0x05010400u);
+          hi[j] = __builtin_amdgcn_perm(y, x, 0x07030602u);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t f[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            f[j] = f16_of_biased(__builtin_amdgcn_perm(0x64646464u, e < 2 ? lo[j] : hi[j], e & 1 ? 0x04030402u : 0x04010400u));
+          const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, make_uint4(f[0], f[1], f[2], f[3]));
+          a8_f32x4 &o = O[4 * i + e];
           o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph8, o, 0, 0, 0);
           if (SPLIT) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl8, o, 0, 0, 0);
-        };
-        step(O[4 * i + 0], make_uint4(f16_of_bytes<0>(w[0], w[1]), f16_of_bytes<0>(w[2], w[3]),
-                                      f16_of_bytes<0>(w[4], w[5]), f16_of_bytes<0>(w[6], w[7])));
-        step(O[4 * i + 1], make_uint4(f16_of_bytes<1>(w[0], w[1]), f16_of_bytes<1>(w[2], w[3]),
-                                      f16_of_bytes<1>(w[4], w[5]), f16_of_bytes<1>(w[6], w[7])));
-        step(O[4 * i + 2], make_uint4(f16_of_bytes<2>(w[0], w[1]), f16_of_bytes<2>(w[2], w[3]),
-                                      f16_of_bytes<2>(w[4], w[5]), f16_of_bytes<2>(w[6], w[7])));
-        step(O[4 * i + 3], make_uint4(f16_of_bytes<3>(w[0], w[1]), f16_of_bytes<3>(w[2], w[3]),
-                                      f16_of_bytes<3>(w[4], w[5]), f16_of_bytes<3>(w[6], w[7])));
+        }
       }
+    }
+  };
+  {
+    constexpr int STEP = CHUNK * NW;
+    int k0 = klo + CHUNK * wave, ids[NT];
+    Chunk c0, c1;
+    if (k0 < khi) {
+      pages(k0, ids);
+      load(k0, ids, c0);
+      pages(k0 + STEP, ids);
+    }
+    // (each call of work() comes behind a load that is certain, so that it
+    // waits for its own chunk's loads alone)
+    while (k0 < khi) {
+      if (k0 + STEP >= khi) {
+        work(k0, c0);
+        break;
+      }
+      load(k0 + STEP, ids, c1);
+      pages(k0 + 2 * STEP, ids);
+      work(k0, c0);
+      k0 += STEP;
+      if (k0 + STEP >= khi) {
+        work(k0, c1);
+        break;
+      }
+      load(k0 + STEP, ids, c0);
+      pages(k0 + 2 * STEP, ids);
+      work(k0, c1);
+      k0 += STEP;
     }
   }
 
@@ -241,7 +327,8 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
   float lr = 0.f, o[DPL] = {};
 #pragma unroll
   for (int w = 0; w < NW; w++) {
-    const float c = sm[w][r] == -INFINITY ? 0.f : exp2_raw(sm[w][r] - Mr);
+    // (-inf: nothing seen, zeros; or NaN scores alone, NaN)
+    const float c = sm[w][r] == -INFINITY ? 1.f : exp2_raw(sm[w][r] - Mr);
     lr = fmaf(sl[w][r], c, lr);
 #pragma unroll
     for (int e = 0; e < DPL; e++) o[e] = fmaf(so[w][r][d + e], c, o[e]);
@@ -274,27 +361,27 @@ __global__ __launch_bounds__(ROWS_THREADS) void k_attn_kv8_rows(AttnArgs a) {
 // banks.  V: step s, tile e, lane l at slot (s DT + e) 64 + l holds the 8 keys
 // above of dim DT r + e; the thread that loads DT neighbouring bytes of those
 // 8 rows writes one slot of each tile.
-// The largest score may run ahead of M by 1.9 before O and l are scaled again, so
-// weights stay under 2^15.9, inside f16.
 constexpr int TILE_ROWS = ATTN_TILE_ROWS, TILE_THREADS = 512;
 typedef float a8_f32x16 __attribute__((ext_vector_type(16)));
 
 template <class T, int HD>
 __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) {
   constexpr bool SPLIT = std::is_same<T, float>::value;
-  constexpr int KS = HD / 16, DT = HD / 32, CPK = HD / 16, KL = 64 * CPK / 256;
-  constexpr float SHIFT = 14.f, AHEAD = 1.9f;
+  constexpr int KS = HD / 16, DT = HD / 32, CPK = HD / 16, KL = 64 * CPK / 256, AHEAD_K = 4;
   static_assert(DT == 2 || DT == 4, "head_dim 64 or 128");
   __shared__ __align__(16) uint4 kl[2][2 * KS * 64], vl[2][4 * DT * 64];
   __shared__ float4 scl[2][4];  // of 16 keys: ks, log2 vs, 1 / vs
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, u = lane >> 5;
-  // heads fastest: the blocks of one KV head's rows go to the same XCDs
-  const int kh = blockIdx.x % a.n_kv, bx = blockIdx.x / a.n_kv, b = blockIdx.y;
-  const int tile = bx / a.tparts, part = bx % a.tparts;
+  // Heads fastest, then a request's tiles, the last ones, which have the most
+  // keys, first: the blocks of one request and KV head run together, on the
+  // same XCDs, and share K and V in their L2 (requests before tiles: 775 ->
+  // 1087 us for 12 requests of 32 tiles and less).
+  const int kh = blockIdx.x % a.n_kv, bx = blockIdx.x / a.n_kv, step = bx % (a.ttiles * a.tparts);
+  const int b = bx / (a.ttiles * a.tparts), tile = a.ttiles - 1 - step / a.tparts, part = step % a.tparts;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
   const int64_t all = (int64_t)rq.fresh * a.group;
-  if (all <= ATTN_FEW_ROWS || (int64_t)tile * TILE_ROWS >= all) return;
+  if (all <= a.few || (int64_t)tile * TILE_ROWS >= all) return;
   const int row0 = tile * TILE_ROWS, rows = (int)min(all - row0, (int64_t)TILE_ROWS);
   const AttnKeys ak = attn_keys(rq, row0 / a.group, (row0 + rows - 1) / a.group, a.window);
   const int nparts = attn_parts(ak, a.tsplit);
@@ -332,50 +419,71 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
       }
   }
   const int see_hi = mine ? rq.first + mytok : -1;
-  const int64_t see_lo = a.window ? (int64_t)see_hi - a.window : -1;
+  const int see_lo = first_hidden(see_hi, a.window);
   // what the wave's rows see together (all: every row sees it)
   const int w0 = row0 + min(32 * wave, rows - 1), w1 = row0 + min(32 * wave + 31, rows - 1);
   const int any_hi = 32 * wave < rows ? rq.first + w1 / a.group : -1, all_hi = rq.first + w0 / a.group;
-  const int64_t any_lo = a.window ? (int64_t)all_hi - a.window : -1, all_lo = a.window ? (int64_t)any_hi - a.window : -1;
+  const int any_lo = first_hidden(all_hi, a.window), all_lo = first_hidden(any_hi, a.window);
   const bool full = 32 * wave + 31 < rows;
 
-  // staging: waves 0..3 take K (KL vectors each), 4..7 V (8 rows of 4 bytes)
+  // Staging: waves 0..3 take K (KL vectors a lane), wave 4 + q the V rows (8 of
+  // them, 4 bytes each, a lane) and scales of 16-key block q.  A wave's vectors
+  // j are of one block, so pages and addresses are scalars; ids are loaded two
+  // chunks ahead, codes one.
   const int *table = a.tables + (int64_t)b * a.wide;
-  const bool isv = tid >= 256;
-  const int t = tid & 255;
-  const int vset = t / (HD / 4), vq = t % (HD / 4), vs16 = vset >> 1, vu = vset & 1;
-  const bool vwork = isv && vset < 8, swork = vwork && vq == 0 && vu == 0;
-  auto block_of = [&](int k0, int j) { return (k0 >> 4) + (isv ? vs16 : (t + 256 * j) / CPK / 16); };
-  auto page_id = [&](int blk) {  // -1: no page, or no key of the part
-    if (16 * blk >= khi) return -1;
-    const int id = table[(int)a.div_page(blk)];
-    return id >= 0 && id < a.n_pages ? id : -1;
-  };
-  int ids[KL], now[KL];
+  const bool isv = wave >= 4;
+  const int t = tid & 255, p16 = a.page >> 4, last_blk = (khi - 1) >> 4, last_pj = a.div_page(last_blk);
+  const int adv = a.div_page(4), rem = 4 - adv * p16;  // a chunk's pages and blocks
+  const int vq = lane % (HD / 4), vu = lane / (HD / 4);  // (head_dim 64: half the lanes)
+  const int lane_off = isv ? 4 * vu * HD + 4 * vq : (t / CPK & 15) * HD + 16 * (t % CPK);
+  const bool vwork = vu < 2;
+  int blk[KL], pj[KL], off[KL], id[KL], next_id[KL];
+#pragma unroll
+  for (int j = 0; j < KL; j++) {
+    blk[j] = (klo >> 4) + (isv ? wave - 4 : KL == 2 ? (wave >> 1) + 2 * j : wave);
+    pj[j] = a.div_page(blk[j]);
+    off[j] = blk[j] - pj[j] * p16;
+  }
   uint4 raw[2];
   float s_k = 0.f, s_v = 0.f;
-  auto load = [&](int k0) {  // codes of the chunk at k0, from pages `now`
-    if (!isv) {
+  bool s_ok = false;
+  auto load = [&]() {  // the codes at blk, from pages id; then on to the next chunk
+    const int8_t *codes = isv ? a.vc : a.kc;
 #pragma unroll
-      for (int j = 0; j < KL; j++) {
-        const int v = t + 256 * j, blk = block_of(k0, j), pj = a.div_page(blk);
-        const int64_t ph = (int64_t)max(now[j], 0) * a.n_kv + kh;
-        const int off = 16 * (blk - pj * (a.page >> 4)) + (v / CPK & 15);
-        raw[j] = *(const uint4 *)(a.kc + (ph * a.page + off) * HD + 16 * (v % CPK));
-      }
-    } else if (vwork) {
-      const int blk = block_of(k0, 0), pj = a.div_page(blk);
-      const int64_t ph = (int64_t)max(now[0], 0) * a.n_kv + kh;
-      const int8_t *p = a.vc + (ph * a.page + 16 * (blk - pj * (a.page >> 4)) + 4 * vu) * HD + 4 * vq;
-      uint32_t w[8];
+    for (int j = 0; j < KL; j++) {
+      if (j == 0 || !isv) {
+        const bool ok = blk[j] <= last_blk && (uint32_t)id[j] < (uint32_t)a.n_pages;
+        // (else page 0's rows are read and not used)
+        const int64_t ph = (int64_t)(ok ? id[j] : 0) * a.n_kv + kh;
+        const int8_t *p = codes + (ph * a.page + 16 * off[j]) * HD;
+        if (!isv) {
+          raw[j] = *(const uint4 *)(p + lane_off);
+        } else {
+          if (vwork) {
+            uint32_t w[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) w[j] = *(const uint32_t *)(p + (j < 4 ? j : j + 4) * HD);
-      raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
-      raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      if (swork) {
-        s_k = a.ks[ph];
-        s_v = a.vs[ph];
+            for (int i = 0; i < 8; i++) w[i] = *(const uint32_t *)(p + lane_off + (i < 4 ? i : i + 4) * HD);
+            raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+          s_k = a.ks[ph];
+          s_v = a.vs[ph];
+          s_ok = ok;
+        }
+        blk[j] += 4;
+        pj[j] += adv;
+        off[j] += rem;
+        const bool wrap = off[j] >= p16;
+        pj[j] += wrap ? 1 : 0;
+        off[j] -= wrap ? p16 : 0;
       }
+    }
+  };
+  auto pages = [&](int (&ids)[KL], int ahead) {  // of the chunk at pj (ahead 1: the one behind it)
+#pragma unroll
+    for (int j = 0; j < KL; j++) {
+      const int at = pj[j] + (ahead ? adv + (off[j] + rem >= p16 ? 1 : 0) : 0);
+      ids[j] = table[min(at, last_pj)];
     }
   };
   auto store = [&](int buf) {
@@ -392,19 +500,29 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
         p[(key & 31) ^ (2 * c & 15)] = lo;
         p[32 + ((key & 31) ^ (2 * c & 15))] = hi;
       }
-    } else if (vwork) {
-      const uint32_t w[8] = {raw[0].x ^ 0x80808080u, raw[0].y ^ 0x80808080u, raw[0].z ^ 0x80808080u, raw[0].w ^ 0x80808080u,
-                             raw[1].x ^ 0x80808080u, raw[1].y ^ 0x80808080u, raw[1].z ^ 0x80808080u, raw[1].w ^ 0x80808080u};
-      // byte e of the 8 rows is dim 4 vq + e: row (4 vq + e) / DT of tile (4 vq + e) % DT
-      auto put = [&](int e, uint4 f) {
-        const int d = 4 * vq + e;
-        vl[buf][(vs16 * DT + d % DT) * 64 + 32 * vu + d / DT] = f;
-      };
-      put(0, make_uint4(f16_of_bytes<0>(w[0], w[1]), f16_of_bytes<0>(w[2], w[3]), f16_of_bytes<0>(w[4], w[5]), f16_of_bytes<0>(w[6], w[7])));
-      put(1, make_uint4(f16_of_bytes<1>(w[0], w[1]), f16_of_bytes<1>(w[2], w[3]), f16_of_bytes<1>(w[4], w[5]), f16_of_bytes<1>(w[6], w[7])));
-      put(2, make_uint4(f16_of_bytes<2>(w[0], w[1]), f16_of_bytes<2>(w[2], w[3]), f16_of_bytes<2>(w[4], w[5]), f16_of_bytes<2>(w[6], w[7])));
-      put(3, make_uint4(f16_of_bytes<3>(w[0], w[1]), f16_of_bytes<3>(w[2], w[3]), f16_of_bytes<3>(w[4], w[5]), f16_of_bytes<3>(w[6], w[7])));
-      if (swork) scl[buf][vs16] = now[0] < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(s_k, log2f(s_v), 1.f / s_v, 0.f);
+    } else {
+      const int q = wave - 4;
+      if (vwork) {
+        // rows in pairs: bytes a0 b0 a1 b1 and a2 b2 a3 b3 of rows a, b; byte e of the
+        // 8 is dim 4 vq + e: row (4 vq + e) / DT of tile (4 vq + e) % DT
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t x = w[2 * j] ^ 0x80808080u, y = w[2 * j + 1] ^ 0x80808080u;
+          lo[j] = __builtin_amdgcn_perm(y, x, 0x05010400u);
+          hi[j] = __builtin_amdgcn_perm(y, x, 0x07030602u);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t f[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            f[j] = f16_of_biased(__builtin_amdgcn_perm(0x64646464u, e < 2 ? lo[j] : hi[j], e & 1 ? 0x04030402u : 0x04010400u));
+          vl[buf][(q * DT + e % DT) * 64 + 32 * vu + (4 / DT) * vq + e / DT] = make_uint4(f[0], f[1], f[2], f[3]);
+        }
+      }
+      if (lane == 0) scl[buf][q] = s_ok ? make_float4(s_k, log2_raw(s_v), rcp_raw(s_v), 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
     }
   };
 
@@ -415,24 +533,29 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
 #pragma unroll
     for (int i = 0; i < 16; i++) O[e][i] = 0.f;
 
-#pragma unroll
-  for (int j = 0; j < KL; j++) now[j] = page_id(block_of(klo, j));
-  if (klo < khi) load(klo);
-#pragma unroll
-  for (int j = 0; j < KL; j++) ids[j] = page_id(block_of(klo + 64, j));
+  if (klo < khi) {
+    pages(id, 0);
+    pages(next_id, 1);
+    load();
+  }
   int buf = 0;
   for (int k0 = klo; k0 < khi; k0 += 64, buf ^= 1) {
+#pragma unroll
+    for (int j = 0; j < KL; j++) id[j] = next_id[j];
+    pages(next_id, 1);
     store(buf);
-    if (k0 + 64 < khi) {
-#pragma unroll
-      for (int j = 0; j < KL; j++) now[j] = ids[j];
-      load(k0 + 64);
-#pragma unroll
-      for (int j = 0; j < KL; j++) ids[j] = page_id(block_of(k0 + 128, j));
-    }
+    if (k0 + 64 < khi) load();
     __syncthreads();
     if (k0 > any_hi || k0 + 63 <= any_lo) continue;
     a8_f32x16 z[2];
+    uint4 vf[2][DT];
+    float4 sc[4];
+    auto vread = [&](int s) {
+#pragma unroll
+      for (int e = 0; e < DT; e++) vf[s & 1][e] = vl[buf][(s * DT + e) * 64 + lane];
+    };
+#pragma unroll
+    for (int q = 0; q < 4; q++) sc[q] = scl[buf][q];
     float mx = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
@@ -445,54 +568,86 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
         if (SPLIT) z[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[ks], z[kt], 0, 0, 0);
       }
     }
+    // LDS reads run ahead of the products (left to itself the compiler waits for
+    // each one)
+    vread(0);
+    sched_ds<4 + AHEAD_K>();  // (the scales, and the first of K)
+#pragma unroll
+    for (int i = 0; i < 2 * KS - AHEAD_K; i++) {
+      sched_mfma<SPLIT ? 2 : 1>();
+      sched_ds<1>();
+    }
+    sched_ds<DT>();
+    sched_mfma<(SPLIT ? 2 : 1) * AHEAD_K>();
     float ivs[4];
     const bool seen = full && k0 + 63 <= all_hi && k0 > all_lo;  // by every row
+    // z - (M - SHIFT), with the M so far: only a row whose scores run ahead of it,
+    // or that has none yet, takes a new one
+    float base = M == -INFINITY ? 0.f : M - SHIFT;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      const float4 sc = scl[buf][q];
-      const float f = sc.x * qf;
-      ivs[q] = sc.z;
+      const float f = sc[q].x * qf, lv = sc[q].y - base;
+      ivs[q] = sc[q].z;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        float x = fmaf(z[q >> 1][8 * (q & 1) + i], f, sc.y);
-        if (!seen) {
-          const int64_t key = k0 + 16 * q + 8 * (i >> 2) + 4 * u + (i & 3);
-          if (!(key <= see_hi && key > see_lo && sc.y != -INFINITY)) x = -INFINITY;
+      for (int i = 0; i < 8; i++) z[q >> 1][8 * (q & 1) + i] = fmaf(z[q >> 1][8 * (q & 1) + i], f, lv);
+    }
+    if (!seen) {
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int key = k0 + 16 * q + 8 * (i >> 2) + 4 * u + (i & 3);
+          if (!(key <= see_hi && key > see_lo && sc[q].y != -INFINITY)) z[q >> 1][8 * (q & 1) + i] = -INFINITY;
         }
-        z[q >> 1][8 * (q & 1) + i] = x;
-        mx = fmaxf(mx, x);
+        // (a page that the row does not see adds nothing, whatever its scale)
+        if (k0 + 16 * q > see_hi || k0 + 16 * q + 15 <= see_lo) ivs[q] = 0.f;
       }
     }
+#pragma unroll
+    for (int i = 0; i < 16; i++) mx = fmaxf(mx, fmaxf(z[0][i], z[1][i]));
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    const bool more = mx > M + AHEAD;
+    const bool more = mx > SHIFT + AHEAD || (M == -INFINITY && mx > -INFINITY);
     if (__any(more)) {
-      const float Mn = more ? mx : M, alpha = !more ? 1.f : M == -INFINITY ? 0.f : exp2_raw(M - Mn);
+      const float Mn = more ? mx + base : M, alpha = !more ? 1.f : M == -INFINITY ? 0.f : exp2_raw(M - Mn);
+      const float by = more ? mx - SHIFT : 0.f;
       M = Mn;
       l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        z[0][i] -= by;
+        z[1][i] -= by;
+      }
 #pragma unroll
       for (int e = 0; e < DT; e++)
 #pragma unroll
         for (int i = 0; i < 16; i++) O[e][i] *= alpha;
     }
-    const float base = M == -INFINITY ? 0.f : M - SHIFT;
-#pragma unroll
-    for (int s = 0; s < 4; s++) {
-      a8_f16x8 ph8, pl8;
+    // Step s: its products, with the weights and V of step s + 1 made meanwhile.
+    a8_f16x8 ph8[2], pl8[2];
+    auto weights = [&](int s) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float p = exp2_raw(z[s >> 1][8 * (s & 1) + j] - base);
-        // (a key that is not seen adds nothing, whatever its page's scale)
-        l = fmaf(p, !seen && p == 0.f ? 0.f : ivs[s], l);
-        ph8[j] = (_Float16)p;
-        if (SPLIT) pl8[j] = (_Float16)(p - (float)ph8[j]);
+        const float p = exp2_raw(z[s >> 1][8 * (s & 1) + j]);
+        l = fmaf(p, ivs[s], l);
+        ph8[s & 1][j] = (_Float16)p;
+        if (SPLIT) pl8[s & 1][j] = (_Float16)(p - (float)ph8[s & 1][j]);
+      }
+    };
+    weights(0);
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      if (s < 3) {
+        vread(s + 1);
+        weights(s + 1);
       }
 #pragma unroll
       for (int e = 0; e < DT; e++) {
-        const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, vl[buf][(s * DT + e) * 64 + lane]);
-        O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph8, O[e], 0, 0, 0);
-        if (SPLIT) O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl8, O[e], 0, 0, 0);
+        const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, vf[s & 1][e]);
+        O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph8[s & 1], O[e], 0, 0, 0);
+        if (SPLIT) O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl8[s & 1], O[e], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   {
@@ -518,18 +673,21 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
     for (int e = 0; e < DT; e++) op[DT * (8 * (i / 4) + 4 * u + i % 4) + e] = (T)(l == 0.f ? 0.f : O[e][i] / l);
 }
 
-// The parts of a row joined: o = sum_p O_p 2^(M_p - M) / sum_p l_p 2^(M_p - M).
-// A wave is one row; rows of one part are written already.
-constexpr int JOIN_THREADS = 256;
-template <class T, int HD>
+// The parts of a row joined: o = sum_p O_p 2^(M_p - M) / sum_p l_p 2^(M_p - M);
+// rows of one part are written already.  WPR waves take a row's parts in turn
+// (1 where there are few, so that a block has 4 rows: 14336 rows of 4 parts in
+// 10 us), 4 of them at once in flight.
+constexpr int JOIN_THREADS = 256, JOIN_FEW = 8;
+template <class T, int HD, int WPR>
 __global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
-  constexpr int LD = HD + 4, DPL = HD / 64;
-  const int lane = threadIdx.x & 63, kh = blockIdx.y, b = blockIdx.z;
+  constexpr int LD = HD + 4, DPL = HD / 64, UN = 4;
+  __shared__ float so[WPR][HD], sl[WPR];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % WPR, kh = blockIdx.y, b = blockIdx.z;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
-  const int64_t row = (int64_t)blockIdx.x * (JOIN_THREADS / 64) + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (JOIN_THREADS / 64 / WPR) + wave / WPR;
   const int64_t all = (int64_t)rq.fresh * a.group;
   if (row >= all) return;
-  const bool tiles = a.tparts && all > ATTN_FEW_ROWS;
+  const bool tiles = a.tparts && all > a.few;
   const int height = tiles ? TILE_ROWS : 16, row0 = (int)(row / height * height);  // of its tile
   const AttnKeys ak = attn_keys(rq, row0 / a.group, (int)((min((int64_t)row0 + height, all) - 1) / a.group), a.window);
   const int n = attn_parts(ak, tiles ? a.tsplit : a.split);
@@ -540,12 +698,39 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
   for (int i = lane; i < n; i += 64) M = fmaxf(M, p[(int64_t)i * LD + HD]);
   M = wave_max(M);
   float l = 0.f, o[DPL] = {};
-  for (int i = 0; i < n; i++) {
-    const float *pi = p + (int64_t)i * LD;
-    const float c = pi[HD] == -INFINITY ? 0.f : exp2_raw(pi[HD] - M);
-    l = fmaf(pi[HD + 1], c, l);
+  for (int i0 = w; i0 < n; i0 += UN * WPR) {
+    float v[UN][DPL], mi[UN], li[UN];
 #pragma unroll
-    for (int e = 0; e < DPL; e++) o[e] = fmaf(pi[DPL * lane + e], c, o[e]);
+    for (int j = 0; j < UN; j++) {
+      const int i = i0 + j * WPR;
+      const float *pi = p + (int64_t)min(i, n - 1) * LD;
+      mi[j] = pi[HD];
+      li[j] = pi[HD + 1];
+#pragma unroll
+      for (int e = 0; e < DPL; e++) v[j][e] = pi[DPL * lane + e];
+    }
+#pragma unroll
+    for (int j = 0; j < UN; j++) {
+      if (i0 + j * WPR >= n) break;
+      // (M_p = -inf: nothing seen, zeros; or NaN scores alone, NaN)
+      const float c = mi[j] == -INFINITY ? 1.f : exp2_raw(mi[j] - M);
+      l = fmaf(li[j], c, l);
+#pragma unroll
+      for (int e = 0; e < DPL; e++) o[e] = fmaf(v[j][e], c, o[e]);
+    }
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int e = 0; e < DPL; e++) so[w][DPL * lane + e] = o[e];
+    if (lane == 0) sl[w] = l;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < WPR; k++) {
+      l += sl[k];
+#pragma unroll
+      for (int e = 0; e < DPL; e++) o[e] += so[k][DPL * lane + e];
+    }
   }
   T *op = (T *)a.out + (int64_t)tok * a.out_stride + (int64_t)head * HD + DPL * lane;
 #pragma unroll
@@ -559,16 +744,19 @@ size_t attn_kv8_bytes(int n_tokens, int n_heads, int hd, const AttnCut &c) {
 template <class T, int HD>
 static void attn_launch(const AttnArgs &a, const AttnCut &c, hipStream_t st) {
   if (c.tparts)
-    hipLaunchKernelGGL((k_attn_kv8_tiles<T, HD>), dim3((unsigned)(c.ttiles * c.tparts * a.n_kv), a.n_requests),
+    hipLaunchKernelGGL((k_attn_kv8_tiles<T, HD>), dim3((unsigned)(c.ttiles * c.tparts * a.n_kv * a.n_requests)),
                        dim3(TILE_THREADS), 0, st, a);
   if (c.rtiles)
-    hipLaunchKernelGGL((k_attn_kv8_rows<T, HD>), dim3((unsigned)(c.rtiles * c.rparts), a.n_kv, a.n_requests),
+    hipLaunchKernelGGL((k_attn_kv8_rows<T, HD>), dim3((unsigned)(c.rtiles * c.rparts * a.n_kv * a.n_requests)),
                        dim3(ROWS_THREADS), 0, st, a);
-  if (c.parts > 1) {
-    const int64_t rows = (int64_t)a.max_new * a.group;
-    hipLaunchKernelGGL((k_attn_kv8_join<T, HD>), dim3((unsigned)((rows + 3) / 4), a.n_kv, a.n_requests), dim3(JOIN_THREADS), 0,
-                       st, a);
-  }
+  // rows that may have parts: all, or where the long tiles have one, the few
+  const int64_t all = (int64_t)a.max_new * a.group;
+  const int64_t rows = c.tparts > 1 ? all : c.rparts > 1 ? std::min<int64_t>(all, c.tparts ? c.few : all) : 0;
+  if (rows && c.parts > JOIN_FEW)
+    hipLaunchKernelGGL((k_attn_kv8_join<T, HD, 4>), dim3((unsigned)rows, a.n_kv, a.n_requests), dim3(JOIN_THREADS), 0, st, a);
+  else if (rows)
+    hipLaunchKernelGGL((k_attn_kv8_join<T, HD, 1>), dim3((unsigned)((rows + 3) / 4), a.n_kv, a.n_requests), dim3(JOIN_THREADS),
+                       0, st, a);
 }
 
 hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, const AttnCut &c, hipStream_t st) {

@@ -342,7 +342,7 @@ struct AttnArgs {
   float scale;
   int n_pages, page, n_kv, group, n_tokens, n_requests, wide, window;
   int max_new, max_ctx;
-  int split, rparts, tsplit, tparts, parts;  // AttnCut
+  int rtiles, ttiles, few, split, rparts, tsplit, tparts, parts;  // AttnCut
   uint32_t page_magic;  // 2^32 / (page / 16) rounded up, 0 for 1
   // page of 16-key block n < 2^27 (n (d - 1) < 2^32, so the product's floor is exact)
   __device__ __forceinline__ int div_page(int n) const { return page_magic ? (int)__umulhi((uint32_t)n, page_magic) : n; }

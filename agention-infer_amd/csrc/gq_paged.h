@@ -91,39 +91,46 @@ GQ_HD int attn_parts(const AttnKeys &k, int split) {
   return k.hi <= k.lo ? 1 : (k.hi - k.lo - 1) / split + 1;
 }
 
-// How a call is cut.  Requests of up to ATTN_FEW_ROWS rows (tokens by query
-// heads of one KV head) take tiles of 16 rows, `rtiles` of them at most, their
-// keys in parts of `split`; the others (tparts 0: there are none) tiles of
+// How a call is cut.  Requests of up to `few` rows (tokens by query heads of
+// one KV head) take tiles of 16 rows, `rtiles` of them at most, their keys in
+// parts of `split`; the others (tparts 0: there are none) tiles of
 // ATTN_TILE_ROWS, ttiles at most, with parts of `tsplit`.  Parts fill the GPU
 // where there are few tiles, and even out requests of different lengths.
 constexpr int ATTN_FEW_ROWS = 64, ATTN_TILE_ROWS = 256;
 struct AttnCut {
   int64_t rtiles, ttiles;
-  int split, rparts, tsplit, tparts;
-  int parts;  // the most of either: the workspace's
+  int few;
+  int split, rparts, tsplit, tparts;  // parts 0: that kernel is not launched
+  int parts;                          // the most of either: the workspace's
 };
-// Parts of a multiple of `step` keys, about `want` of them for max_ctx keys.
-inline void attn_split(int64_t want, int step, int max_ctx, int &split, int &parts) {
-  const int64_t most = ((int64_t)max_ctx + step - 1) / step;
+// max_ctx keys in parts of a multiple of 256, about `want` of them.
+inline void attn_split(int64_t want, int max_ctx, int &split, int &parts) {
+  const int64_t most = ((int64_t)max_ctx + 255) / 256;
   const int64_t n = want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most;
-  int64_t s = (((int64_t)max_ctx + n - 1) / n + step - 1) / step * step;
-  s = s < step ? step : s > (1 << 30) ? (1 << 30) : s;
-  split = (int)s;
-  parts = max_ctx ? (int)(((int64_t)max_ctx + s - 1) / s) : 1;
+  const int64_t s = (((int64_t)max_ctx + n - 1) / n + 255) / 256 * 256;
+  split = (int)(s < 256 ? 256 : s > (1 << 30) ? (1 << 30) : s);
+  parts = max_ctx ? (int)(((int64_t)max_ctx + split - 1) / split) : 1;
 }
 inline AttnCut attn_cut(int n_tokens, int n_requests, int n_kv_heads, int group, int max_new, int max_ctx) {
   AttnCut c{};
   const int64_t rows = (int64_t)max_new * group, heads = (int64_t)n_requests * n_kv_heads;
-  const int64_t few = rows < ATTN_FEW_ROWS ? rows : ATTN_FEW_ROWS;
+  // (one request of many rows: no second launch for the few)
+  c.few = rows > ATTN_FEW_ROWS && n_requests == 1 ? 0 : ATTN_FEW_ROWS;
+  const int64_t few = rows < c.few ? rows : c.few;
   c.rtiles = (few + 15) / 16;
-  attn_split(heads ? 4096 / (heads * (c.rtiles ? c.rtiles : 1)) : 1, 256, max_ctx, c.split, c.rparts);
-  c.parts = c.rparts;
+  if (c.rtiles) {
+    // two blocks a CU at least; with enough work parts of 1024 keys (4 chunks
+    // a wave) or so
+    const int64_t blocks = heads ? heads * c.rtiles : 1, k = ((int64_t)max_ctx + 1023) / 1024;
+    attn_split(blocks * k >= 512 ? k : (512 + blocks - 1) / blocks, max_ctx, c.split, c.rparts);
+    c.parts = c.rparts;
+  }
   if (rows > ATTN_FEW_ROWS) {
     c.ttiles = (rows + ATTN_TILE_ROWS - 1) / ATTN_TILE_ROWS;
     // (of ragged requests: no more than the pass's rows make, and a partial one each)
     const int64_t whole = (int64_t)n_tokens * group / ATTN_TILE_ROWS + n_requests;
     const int64_t tiles = n_kv_heads * (c.ttiles * n_requests < whole ? c.ttiles * n_requests : whole);
-    attn_split(tiles ? 256 / tiles : 1, 256, max_ctx, c.tsplit, c.tparts);
+    attn_split(tiles ? 256 / tiles : 1, max_ctx, c.tsplit, c.tparts);
     c.parts = c.parts > c.tparts ? c.parts : c.tparts;
   }
   return c;

@@ -5,8 +5,8 @@
 //   owner N V AT0 .. ATN  ->  owner_of
 //   req S E CTX N WIDE PAGE MAXCTX  ->  start fresh first keys of attn_request
 //   keys FRESH FIRST KEYS I0 I1 WINDOW SPLIT  ->  lo hi of attn_keys, attn_parts
-//   cut TOKENS REQUESTS KV GROUP MAXNEW MAXCTX  ->  rtiles split rparts ttiles tsplit
-//                                               tparts parts of attn_cut
+//   cut TOKENS REQUESTS KV GROUP MAXNEW MAXCTX  ->  few rtiles split rparts ttiles
+//                                               tsplit tparts parts of attn_cut
 #include <cstdio>
 #include <cstring>
 #include <vector>
@@ -43,7 +43,7 @@ int main() {
       int n, nr, kv, group, fresh, ctx;
       if (std::scanf("%d %d %d %d %d %d", &n, &nr, &kv, &group, &fresh, &ctx) != 6) return 1;
       const gq::AttnCut t = gq::attn_cut(n, nr, kv, group, fresh, ctx);
-      std::printf("%lld %d %d %lld %d %d %d\n", (long long)t.rtiles, t.split, t.rparts, (long long)t.ttiles, t.tsplit,
+      std::printf("%d %lld %d %d %lld %d %d %d\n", t.few, (long long)t.rtiles, t.split, t.rparts, (long long)t.ttiles, t.tsplit,
                   t.tparts, t.parts);
     } else {
       return 1;

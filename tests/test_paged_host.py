@@ -263,11 +263,14 @@ def test_attention_cut(ask):
     """Every row has a tile and every key a part, whatever the sizes."""
     cases = [(n, r, kv, g, m, c) for n in (1, 700, 2**31 - 1) for r in (1, 3, 64, 65535) for kv in (1, 8) for g in (1, 7, 71)
              for m in (1, 5, 2048) for c in (0, 1, 255, 4097, 131072, 2**31 - 1)]
-    for (n, r, kv, g, m, c), (rtiles, split, rparts, ttiles, tsplit, tparts, parts) in zip(
+    for (n, r, kv, g, m, c), (most, rtiles, split, rparts, ttiles, tsplit, tparts, parts) in zip(
             cases, ask(["cut " + " ".join(map(str, x)) for x in cases])):
-        few = min(m * g, 64)
-        assert 16 * rtiles >= few > 16 * (rtiles - 1)
-        assert split % 64 == 0 and split > 0 and rparts >= 1 and rparts * split >= c and (rparts - 1) * split < max(c, 1)
+        few = min(m * g, most)
+        assert (most == 64 or m * g > 64 and r == 1 and most == 0) and 16 * rtiles >= few > 16 * (rtiles - 1)
+        if few:
+            assert split % 64 == 0 and split > 0 and rparts >= 1 and rparts * split >= c and (rparts - 1) * split < max(c, 1)
+        else:
+            assert rparts == 0
         if m * g > 64:
             assert 256 * ttiles >= m * g > 256 * (ttiles - 1)
             assert tsplit % 64 == 0 and tsplit > 0 and tparts * tsplit >= c and (tparts - 1) * tsplit < max(c, 1)
