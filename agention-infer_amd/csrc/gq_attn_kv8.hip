@@ -53,11 +53,17 @@ __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp
 __device__ __forceinline__ float log2_raw(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_raw(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// What the instruction scheduler puts next (LDS reads, matrix instructions).
+// What the instruction scheduler puts next: LDS reads and writes, matrix and other
+// vector instructions.
 template <int N>
 __device__ __forceinline__ void sched_ds() { __builtin_amdgcn_sched_group_barrier(0x100, N, 0); }
 template <int N>
 __device__ __forceinline__ void sched_mfma() { __builtin_amdgcn_sched_group_barrier(0x008, N, 0); }
+
+template <int N>
+__device__ __forceinline__ void sched_valu() { __builtin_amdgcn_sched_group_barrier(0x002, N, 0); }
+template <int N>
+__device__ __forceinline__ void sched_dsw() { __builtin_amdgcn_sched_group_barrier(0x200, N, 0); }
 
 // The last position in front of what a row at `pos` sees.
 __device__ __forceinline__ int first_hidden(int pos, int window) {
@@ -131,8 +137,9 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
       if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
     }
   // keys that row m sees: (see_lo, see_hi]; all_lo, all_hi: that each row sees
-  const int see_hi = m < rows ? rq.first + mytok : -1;
-  const int see_lo = first_hidden(see_hi, a.window), all_hi = rows == 16 ? rq.first + row0 / a.group : -1;
+  const int see_hi = m < rows ? min(rq.first + mytok, rq.keys - 1) : -1;
+  const int see_lo = first_hidden(rq.first + mytok, a.window);
+  const int all_hi = rows == 16 ? min(rq.first + row0 / a.group, rq.keys - 1) : -1;
   const int all_lo = first_hidden(rq.first + (row0 + rows - 1) / a.group, a.window);
 
   float M = -INFINITY, l = 0.f;
@@ -348,9 +355,8 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
 
 // ------------------------------------------------------------ long tiles
 // A block is 256 query rows of a (request, KV head) over one part of its keys:
-// 8 waves of 32 rows that share chunks of 64 keys in LDS, as f16, two buffers,
-// one barrier a chunk; the codes of the next chunk are on their way in
-// registers meanwhile.  On v_mfma_f32_32x32x16_f16, transposed as above:
+// 8 waves of 32 rows that share chunks of 64 keys in LDS, as f16.  On
+// v_mfma_f32_32x32x16_f16, transposed as above:
 //   S^T  lane (r = lane % 32, u = lane / 32): keys 8 (i / 4) + 4 u + i % 4 of each
 //        32, of row r.  A row's softmax is its lane's 32 values and one swap.
 //   O^T  depth step s takes the lane's values 8 s' .. 8 s' + 7, that is keys
@@ -359,18 +365,37 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
 // lane.  K: step ks (dims 16 ks ..) of key tile kt, lane l at slot
 // (kt KS + ks) 64 + (l ^ 2 ks): the swap spreads the writes of a key's row over the
 // banks.  V: step s, tile e, lane l at slot (s DT + e) 64 + l holds the 8 keys
-// above of dim DT r + e; the thread that loads DT neighbouring bytes of those
-// 8 rows writes one slot of each tile.
+// above of dim DT r + e.
+//
+// A SIMD has two of the waves, one of each half.  A wave's turn has a matrix
+// half (O of the last chunk, S of this one, and between those instructions the
+// conversion of the chunk after next and the loads of the one behind it) and a
+// vector half (softmax), and the halves of the block are one of them apart, so
+// that one wave's matrix instructions run beside the other's exponentials.  So
+// K lives in 3 buffers and V in 4: chunk n + 2 is written while n - 1 .. n + 1 are read.
 constexpr int TILE_ROWS = ATTN_TILE_ROWS, TILE_THREADS = 512;
 typedef float a8_f32x16 __attribute__((ext_vector_type(16)));
+
+// (fmaxf would first quiet each operand: an instruction more each)
+__device__ __forceinline__ float max3_raw(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 
 template <class T, int HD>
 __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) {
   constexpr bool SPLIT = std::is_same<T, float>::value;
-  constexpr int KS = HD / 16, DT = HD / 32, CPK = HD / 16, KL = 64 * CPK / 256, AHEAD_K = 4;
+  constexpr int KS = HD / 16, DT = HD / 32, CPK = HD / 16, DEEP = SPLIT ? 6 : 11, NP = SPLIT ? 2 : 1;
+  constexpr int KB = 3, VB = 4;  // buffers
   static_assert(DT == 2 || DT == 4, "head_dim 64 or 128");
-  __shared__ __align__(16) uint4 kl[2][2 * KS * 64], vl[2][4 * DT * 64];
-  __shared__ float4 scl[2][4];  // of 16 keys: ks, log2 vs, 1 / vs
+  __shared__ __align__(16) struct {
+    uint4 k[KB][2 * KS * 64], v[VB][4 * DT * 64];
+  } kv;
+  auto &kl = kv.k;
+  auto &vl = kv.v;
+  __shared__ float4 scl[VB][4];  // of 16 keys: ks, log2 vs, 1 / vs
+  __shared__ float4 dump[64];    // where the lanes that have no scale to write do
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, u = lane >> 5;
   // Heads fastest, then a request's tiles, the last ones, which have the most
@@ -387,7 +412,99 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
   const int nparts = attn_parts(ak, a.tsplit);
   if (part >= nparts) return;
   const int klo = ak.lo + part * a.tsplit, khi = (int)min((int64_t)ak.hi, (int64_t)klo + a.tsplit);
+  const int chunks = khi > klo ? (khi - klo + 63) >> 6 : 0;
   const int nh = a.n_kv * a.group;
+
+  // Staging.  A wave takes 8 keys of K (16 bytes a lane) and the V rows 4 u' + 8 (wave % 2)
+  // .. + 3 of the same 16-key block wave / 2 (4 dims by 4 keys a lane; with head_dim
+  // 64 the upper lanes repeat the lower), so pages and addresses are scalars.  The
+  // page's id is loaded two chunks ahead of its codes' use, by a vector load as the
+  // scales (a scalar load in flight would be waited for at every LDS read).
+  const int *table = a.tables + (int64_t)b * a.wide;
+  const int p16 = a.page >> 4, last_blk = max(khi - 1, 0) >> 4, last_pj = a.div_page(last_blk);
+  const int adv = a.div_page(4), rem = 4 - adv * p16;  // a chunk's pages and blocks
+  const int tk = HD == 128 ? tid : 32 * wave + (lane & 31);
+  const int kkey = tk / CPK, kc = tk % CPK, vq = lane % (HD / 4), vu = lane / (HD / 4) & 1, vhf = wave & 1, q16 = wave >> 1;
+  const int koff = (kkey & 15) * HD + 16 * kc, voff = (4 * vu + 8 * vhf) * HD + 4 * vq;
+  const uint32_t stride = (uint32_t)a.n_kv * a.page * HD;  // bytes of a page
+  const int8_t *kbase = a.kc + (int64_t)kh * a.page * HD, *vbase = a.vc + (int64_t)kh * a.page * HD;
+  int vz = 0;
+  asm volatile("" : "+v"(vz));
+  int blk = (klo >> 4) + q16, pj = a.div_page(blk), off = blk - pj * p16, id = 0, next_id = 0;
+  struct Raw {
+    uint4 k;
+    uint32_t v[4];
+    float ks, vs;
+    int ok;
+  };
+  // the id of the page behind that of the block at pj (ahead: by one more chunk)
+  auto page_id = [&](bool ahead) {
+    const int at = ahead ? pj + adv + (off + rem >= p16 ? 1 : 0) : pj;
+    return table[min(at, last_pj) + vz];
+  };
+  auto load = [&](Raw &w) {  // the chunk at blk; then on to the next (past the last: page 0, not used)
+    const int pid = __builtin_amdgcn_readfirstlane(id);
+    const bool ok = (blk <= last_blk) & ((uint32_t)pid < (uint32_t)a.n_pages);
+    const uint32_t page = ok ? pid : 0;
+    const int64_t at = (int64_t)((uint64_t)page * stride) + off * 16 * HD;
+    const int8_t *kp = kbase + at, *vp = vbase + at;
+    w.k = *(const uint4 *)(kp + koff);
+#pragma unroll
+    for (int i = 0; i < 4; i++) w.v[i] = *(const uint32_t *)(vp + voff + i * HD);
+    w.ks = a.ks[(int)(page * a.n_kv + kh) + vz];
+    w.vs = a.vs[(int)(page * a.n_kv + kh) + vz];
+    w.ok = ok;
+    id = next_id;
+    blk += 4;
+    off += rem;
+    pj += adv;
+    const int wrap = off >= p16;
+    pj += wrap;
+    off -= wrap ? p16 : 0;
+    next_id = page_id(true);
+  };
+  auto store = [&](const Raw &w, int kb, int vb) {
+    uint4 lo, hi;
+    f16_of_dword(w.k.x, lo.x, lo.y);
+    f16_of_dword(w.k.y, lo.z, lo.w);
+    f16_of_dword(w.k.z, hi.x, hi.y);
+    f16_of_dword(w.k.w, hi.z, hi.w);
+    uint4 *p = kl[kb] + ((kkey >> 5) * KS + kc) * 64 + ((kkey & 31) ^ (2 * kc & 15));
+    p[0] = lo;
+    p[32] = hi;
+    // V's rows in pairs: bytes a0 b0 a1 b1 and a2 b2 a3 b3 of rows a, b; byte e of the 4
+    // rows is dim 4 vq + e: row (4 vq + e) / DT of tile (4 vq + e) % DT, its keys half
+    // vhf of the lane's 8
+    uint32_t x[4], m01[2], m23[2];
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = w.v[i] ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      m01[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05010400u);
+      m23[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07030602u);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t sel = e & 1 ? 0x04030402u : 0x04010400u;
+      const uint2 f = make_uint2(f16_of_biased(__builtin_amdgcn_perm(0x64646464u, e < 2 ? m01[0] : m23[0], sel)),
+                                 f16_of_biased(__builtin_amdgcn_perm(0x64646464u, e < 2 ? m01[1] : m23[1], sel)));
+      *((uint2 *)(vl[vb] + (q16 * DT + e % DT) * 64 + 32 * vu + (4 / DT) * vq + e / DT) + vhf) = f;
+    }
+    *(lane == 0 ? &scl[vb][q16] : &dump[lane]) =
+        make_float4(w.ok ? w.ks : 0.f, w.ok ? log2_raw(w.vs) : -INFINITY, w.ok ? rcp_raw(w.vs) : 0.f, 0.f);
+  };
+
+  Raw raw{};
+  if (chunks) {
+    Raw first;
+    id = page_id(false);
+    next_id = page_id(true);
+    load(first);
+    load(raw);
+    store(first, 0, 0);
+    store(raw, 1, 1);
+    load(raw);
+  }
 
   const int myrow = row0 + min(32 * wave + r, rows - 1), mytok = myrow / a.group, myhead = kh * a.group + myrow % a.group;
   const bool mine = 32 * wave + r < rows;
@@ -418,196 +535,91 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
         if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
       }
   }
-  const int see_hi = mine ? rq.first + mytok : -1;
-  const int see_lo = first_hidden(see_hi, a.window);
-  // what the wave's rows see together (all: every row sees it)
-  const int w0 = row0 + min(32 * wave, rows - 1), w1 = row0 + min(32 * wave + 31, rows - 1);
-  const int any_hi = 32 * wave < rows ? rq.first + w1 / a.group : -1, all_hi = rq.first + w0 / a.group;
-  const int any_lo = first_hidden(all_hi, a.window), all_lo = first_hidden(any_hi, a.window);
+  // the row sees keys (see_lo, see_hi], every row of the wave (all_lo, all_hi]
+  const int pos = rq.first + mytok, last = rq.keys - 1;
+  const int pos0 = rq.first + (row0 + min(32 * wave, rows - 1)) / a.group;
+  const int pos1 = rq.first + (row0 + min(32 * wave + 31, rows - 1)) / a.group;
+  const int see_hi = mine ? min(pos, last) : -1, see_lo = first_hidden(pos, a.window);
+  const int all_hi = min(pos0, last), all_lo = first_hidden(pos1, a.window);
   const bool full = 32 * wave + 31 < rows;
 
-  // Staging: waves 0..3 take K (KL vectors a lane), wave 4 + q the V rows (8 of
-  // them, 4 bytes each, a lane) and scales of 16-key block q.  A wave's vectors
-  // j are of one block, so pages and addresses are scalars; ids are loaded two
-  // chunks ahead, codes one.
-  const int *table = a.tables + (int64_t)b * a.wide;
-  const bool isv = wave >= 4;
-  const int t = tid & 255, p16 = a.page >> 4, last_blk = (khi - 1) >> 4, last_pj = a.div_page(last_blk);
-  const int adv = a.div_page(4), rem = 4 - adv * p16;  // a chunk's pages and blocks
-  const int vq = lane % (HD / 4), vu = lane / (HD / 4);  // (head_dim 64: half the lanes)
-  const int lane_off = isv ? 4 * vu * HD + 4 * vq : (t / CPK & 15) * HD + 16 * (t % CPK);
-  const bool vwork = vu < 2;
-  int blk[KL], pj[KL], off[KL], id[KL], next_id[KL];
-#pragma unroll
-  for (int j = 0; j < KL; j++) {
-    blk[j] = (klo >> 4) + (isv ? wave - 4 : KL == 2 ? (wave >> 1) + 2 * j : wave);
-    pj[j] = a.div_page(blk[j]);
-    off[j] = blk[j] - pj[j] * p16;
-  }
-  uint4 raw[2];
-  float s_k = 0.f, s_v = 0.f;
-  bool s_ok = false;
-  auto load = [&]() {  // the codes at blk, from pages id; then on to the next chunk
-    const int8_t *codes = isv ? a.vc : a.kc;
-#pragma unroll
-    for (int j = 0; j < KL; j++) {
-      if (j == 0 || !isv) {
-        const bool ok = blk[j] <= last_blk && (uint32_t)id[j] < (uint32_t)a.n_pages;
-        // (else page 0's rows are read and not used)
-        const int64_t ph = (int64_t)(ok ? id[j] : 0) * a.n_kv + kh;
-        const int8_t *p = codes + (ph * a.page + 16 * off[j]) * HD;
-        if (!isv) {
-          raw[j] = *(const uint4 *)(p + lane_off);
-        } else {
-          if (vwork) {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = *(const uint32_t *)(p + lane_off + (i < 4 ? i : i + 4) * HD);
-            raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            raw[1] = make_uint4(w[4], w[5], w[6], w[7]);
-          }
-          s_k = a.ks[ph];
-          s_v = a.vs[ph];
-          s_ok = ok;
-        }
-        blk[j] += 4;
-        pj[j] += adv;
-        off[j] += rem;
-        const bool wrap = off[j] >= p16;
-        pj[j] += wrap ? 1 : 0;
-        off[j] -= wrap ? p16 : 0;
-      }
-    }
-  };
-  auto pages = [&](int (&ids)[KL], int ahead) {  // of the chunk at pj (ahead 1: the one behind it)
-#pragma unroll
-    for (int j = 0; j < KL; j++) {
-      const int at = pj[j] + (ahead ? adv + (off[j] + rem >= p16 ? 1 : 0) : 0);
-      ids[j] = table[min(at, last_pj)];
-    }
-  };
-  auto store = [&](int buf) {
-    if (!isv) {
-#pragma unroll
-      for (int j = 0; j < KL; j++) {
-        const int v = t + 256 * j, key = v / CPK, c = v % CPK;
-        uint4 lo, hi;
-        f16_of_dword(raw[j].x, lo.x, lo.y);
-        f16_of_dword(raw[j].y, lo.z, lo.w);
-        f16_of_dword(raw[j].z, hi.x, hi.y);
-        f16_of_dword(raw[j].w, hi.z, hi.w);
-        uint4 *p = kl[buf] + ((key >> 5) * KS + c) * 64;
-        p[(key & 31) ^ (2 * c & 15)] = lo;
-        p[32 + ((key & 31) ^ (2 * c & 15))] = hi;
-      }
-    } else {
-      const int q = wave - 4;
-      if (vwork) {
-        // rows in pairs: bytes a0 b0 a1 b1 and a2 b2 a3 b3 of rows a, b; byte e of the
-        // 8 is dim 4 vq + e: row (4 vq + e) / DT of tile (4 vq + e) % DT
-        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-        uint32_t lo[4], hi[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint32_t x = w[2 * j] ^ 0x80808080u, y = w[2 * j + 1] ^ 0x80808080u;
-          lo[j] = __builtin_amdgcn_perm(y, x, 0x05010400u);
-          hi[j] = __builtin_amdgcn_perm(y, x, 0x07030602u);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          uint32_t f[4];
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            f[j] = f16_of_biased(__builtin_amdgcn_perm(0x64646464u, e < 2 ? lo[j] : hi[j], e & 1 ? 0x04030402u : 0x04010400u));
-          vl[buf][(q * DT + e % DT) * 64 + 32 * vu + (4 / DT) * vq + e / DT] = make_uint4(f[0], f[1], f[2], f[3]);
-        }
-      }
-      if (lane == 0) scl[buf][q] = s_ok ? make_float4(s_k, log2_raw(s_v), rcp_raw(s_v), 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
-    }
-  };
-
   float M = -INFINITY, l = 0.f;
-  a8_f32x16 O[DT];
+  a8_f32x16 O[DT], z[2];
 #pragma unroll
   for (int e = 0; e < DT; e++)
 #pragma unroll
     for (int i = 0; i < 16; i++) O[e][i] = 0.f;
+  a8_f16x8 ph8[4], pl8[SPLIT ? 4 : 1];
 
-  if (klo < khi) {
-    pages(id, 0);
-    pages(next_id, 1);
-    load();
-  }
-  int buf = 0;
-  for (int k0 = klo; k0 < khi; k0 += 64, buf ^= 1) {
+  // LDS reads run DEEP ahead of the products (left to itself the compiler waits
+  // for each), the rest of the half is spread between these.
+  // O^T += V^T . P^T of the weights in ph8, pl8
+  auto pv = [&](int vb) {
 #pragma unroll
-    for (int j = 0; j < KL; j++) id[j] = next_id[j];
-    pages(next_id, 1);
-    store(buf);
-    if (k0 + 64 < khi) load();
-    __syncthreads();
-    if (k0 > any_hi || k0 + 63 <= any_lo) continue;
-    a8_f32x16 z[2];
-    uint4 vf[2][DT];
-    float4 sc[4];
-    auto vread = [&](int s) {
+    for (int s = 0; s < 4; s++)
 #pragma unroll
-      for (int e = 0; e < DT; e++) vf[s & 1][e] = vl[buf][(s * DT + e) * 64 + lane];
-    };
+      for (int e = 0; e < DT; e++) {
+        const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, vl[vb][(s * DT + e) * 64 + lane]);
+        O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph8[s], O[e], 0, 0, 0);
+        if (SPLIT) O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl8[s], O[e], 0, 0, 0);
+      }
+  };
+  auto order = [&]() {
+    sched_ds<DEEP>();
 #pragma unroll
-    for (int q = 0; q < 4; q++) sc[q] = scl[buf][q];
-    float mx = -INFINITY;
+    for (int i = 0; i < 4 * DT + 2 * KS - DEEP; i++) {
+      sched_mfma<NP>();
+      sched_ds<1>();
+    }
+    sched_mfma<NP * DEEP>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // S^T of the chunk in K buffer kb
+  auto qk = [&](int kb) {
 #pragma unroll
     for (int kt = 0; kt < 2; kt++) {
 #pragma unroll
       for (int i = 0; i < 16; i++) z[kt][i] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        const a8_f16x8 k8 = __builtin_bit_cast(a8_f16x8, kl[buf][(kt * KS + ks) * 64 + (lane ^ (2 * ks & 15))]);
+        const a8_f16x8 k8 = __builtin_bit_cast(a8_f16x8, kl[kb][(kt * KS + ks) * 64 + (lane ^ (2 * ks & 15))]);
         z[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[ks], z[kt], 0, 0, 0);
         if (SPLIT) z[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[ks], z[kt], 0, 0, 0);
       }
     }
-    // LDS reads run ahead of the products (left to itself the compiler waits for
-    // each one)
-    vread(0);
-    sched_ds<4 + AHEAD_K>();  // (the scales, and the first of K)
-#pragma unroll
-    for (int i = 0; i < 2 * KS - AHEAD_K; i++) {
-      sched_mfma<SPLIT ? 2 : 1>();
-      sched_ds<1>();
-    }
-    sched_ds<DT>();
-    sched_mfma<(SPLIT ? 2 : 1) * AHEAD_K>();
-    float ivs[4];
-    const bool seen = full && k0 + 63 <= all_hi && k0 > all_lo;  // by every row
+  };
+  // z of the chunk at k0 to weights
+  auto softmax = [&](int k0, int vb) {
     // z - (M - SHIFT), with the M so far: only a row whose scores run ahead of it,
     // or that has none yet, takes a new one
-    float base = M == -INFINITY ? 0.f : M - SHIFT;
+    const float base = M == -INFINITY ? 0.f : M - SHIFT;
+    float ivs[4];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      const float f = sc[q].x * qf, lv = sc[q].y - base;
-      ivs[q] = sc[q].z;
+      const float4 sc = scl[vb][q];  // (no page: log2 vs is -inf, and with it z)
+      const float f = sc.x * qf, lv = sc.y - base;
+      ivs[q] = sc.z;
 #pragma unroll
       for (int i = 0; i < 8; i++) z[q >> 1][8 * (q & 1) + i] = fmaf(z[q >> 1][8 * (q & 1) + i], f, lv);
     }
-    if (!seen) {
+    if (!(full && k0 + 63 <= all_hi && k0 > all_lo)) {  // not seen by every row
 #pragma unroll
       for (int q = 0; q < 4; q++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const int key = k0 + 16 * q + 8 * (i >> 2) + 4 * u + (i & 3);
-          if (!(key <= see_hi && key > see_lo && sc[q].y != -INFINITY)) z[q >> 1][8 * (q & 1) + i] = -INFINITY;
+          z[q >> 1][8 * (q & 1) + i] = ((key > see_hi) | (key <= see_lo)) ? -INFINITY : z[q >> 1][8 * (q & 1) + i];
         }
         // (a page that the row does not see adds nothing, whatever its scale)
-        if (k0 + 16 * q > see_hi || k0 + 16 * q + 15 <= see_lo) ivs[q] = 0.f;
+        ivs[q] = ((k0 + 16 * q > see_hi) | (k0 + 16 * q + 15 <= see_lo)) ? 0.f : ivs[q];
       }
     }
+    float mx = fmaxf(z[0][0], z[1][0]);
 #pragma unroll
-    for (int i = 0; i < 16; i++) mx = fmaxf(mx, fmaxf(z[0][i], z[1][i]));
+    for (int i = 1; i < 16; i++) mx = max3_raw(mx, z[0][i], z[1][i]);
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-    const bool more = mx > SHIFT + AHEAD || (M == -INFINITY && mx > -INFINITY);
+    const bool more = (mx > SHIFT + AHEAD) | ((M == -INFINITY) & (mx > -INFINITY));
     if (__any(more)) {
       const float Mn = more ? mx + base : M, alpha = !more ? 1.f : M == -INFINITY ? 0.f : exp2_raw(M - Mn);
       const float by = more ? mx - SHIFT : 0.f;
@@ -623,54 +635,102 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
 #pragma unroll
         for (int i = 0; i < 16; i++) O[e][i] *= alpha;
     }
-    // Step s: its products, with the weights and V of step s + 1 made meanwhile.
-    a8_f16x8 ph8[2], pl8[2];
-    auto weights = [&](int s) {
+#pragma unroll
+    for (int s = 0; s < 4; s++)
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const float p = exp2_raw(z[s >> 1][8 * (s & 1) + j]);
         l = fmaf(p, ivs[s], l);
-        ph8[s & 1][j] = (_Float16)p;
-        if (SPLIT) pl8[s & 1][j] = (_Float16)(p - (float)ph8[s & 1][j]);
+        ph8[s][j] = (_Float16)p;
+        if (SPLIT) pl8[s][j] = (_Float16)(p - (float)ph8[s][j]);
       }
-    };
-    weights(0);
+  };
+  // Weights of no chunk, and the V that they are multiplied with.
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
-      if (s < 3) {
-        vread(s + 1);
-        weights(s + 1);
-      }
+  for (int s = 0; s < 4; s++)
 #pragma unroll
-      for (int e = 0; e < DT; e++) {
-        const a8_f16x8 v8 = __builtin_bit_cast(a8_f16x8, vf[s & 1][e]);
-        O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph8[s & 1], O[e], 0, 0, 0);
-        if (SPLIT) O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl8[s & 1], O[e], 0, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+    for (int j = 0; j < 8; j++) {
+      ph8[s][j] = (_Float16)0.f;
+      if (SPLIT) pl8[s][j] = (_Float16)0.f;
     }
+  for (int i = tid; i < 4 * DT * 64; i += TILE_THREADS) vl[VB - 1][i] = make_uint4(0, 0, 0, 0);
+
+  __syncthreads();
+  if (wave >= 4) __syncthreads();
+  int kb = 0, vb = 0;  // buffers of chunk n
+  auto turn = [&]() {
+    kb = kb == KB - 1 ? 0 : kb + 1;
+    vb = (vb + 1) & (VB - 1);
+  };
+  if (32 * wave >= rows) {  // a wave without rows only stages
+    for (int n = 0; n < chunks; n++) {
+      store(raw, kb ? kb - 1 : KB - 1, vb ^ 2);
+      load(raw);
+      __syncthreads();
+      __syncthreads();
+      turn();
+    }
+  } else {
+    for (int n = 0; n < chunks; n++) {
+      pv((vb + VB - 1) & (VB - 1));
+      qk(kb);
+      store(raw, kb ? kb - 1 : KB - 1, vb ^ 2);  // (kb + 2) % 3, (vb + 2) % 4
+      load(raw);
+      order();
+      __syncthreads();
+      softmax(klo + 64 * n, vb);
+      __syncthreads();
+      turn();
+    }
+    pv((vb + VB - 1) & (VB - 1));
   }
+  if (wave < 4) __syncthreads();
   {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
-  if (!mine) return;
-  // row r's dims DT (8 (i / 4) + 4 u + i % 4) + e
+  // Rows go out through LDS (a wave's own part of it, free behind the barrier), so
+  // that 16 lanes write one run of 256 bytes: lane by lane, 8 bytes in each of 64
+  // rows at once, the block's end took 17000 cycles and more.
+  __syncthreads();
+  static_assert(sizeof(kv) >= 8 * 32 * (2 * HD + 16), "rows of a block");
+  char *mem = (char *)&kv + wave * 32 * (2 * HD + 16);
+  auto rows_out = [&](auto zero, float scale, auto &&at) {  // at(row of the wave): where its HD values go
+    typedef decltype(zero) X;
+    constexpr int VP = HD * 2 / (int)sizeof(X), PASSES = HD / VP, LPR = HD / 8, VE = 16 / (int)sizeof(X);
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+      // row r's dims DT (8 (i / 4) + 4 u + i % 4) + e
+#pragma unroll
+      for (int i = 16 / PASSES * p; i < 16 / PASSES * (p + 1); i++) {
+        Vec<X, DT> w;
+#pragma unroll
+        for (int e = 0; e < DT; e++) w.v[e] = (X)(O[e][i] * scale);
+        *(Vec<X, DT> *)(mem + r * (2 * HD + 16) + (DT * (8 * (i / 4) + 4 * u + i % 4) - VP * p) * sizeof(X)) = w;
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 32 * LPR / 64; k++) {
+        const int row = (64 * k + lane) / LPR, c = lane % LPR;
+        if (32 * wave + row < rows)
+          *(uint4 *)((X *)at(row) + VP * p + VE * c) = *(const uint4 *)(mem + row * (2 * HD + 16) + 16 * c);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  auto token_of = [&](int row) { return (row0 + 32 * wave + row) / a.group; };
+  auto head_of = [&](int row) { return kh * a.group + (row0 + 32 * wave + row) % a.group; };
   if (nparts > 1) {
-    float *p = a.part + (((int64_t)(rq.start + mytok) * nh + myhead) * a.parts + part) * (HD + 4);
-#pragma unroll
-    for (int i = 0; i < 16; i++)
-#pragma unroll
-      for (int e = 0; e < DT; e += 2)
-        *(float2 *)(p + DT * (8 * (i / 4) + 4 * u + i % 4) + e) = make_float2(O[e][i], O[e + 1][i]);
-    if (u == 0) *(float2 *)(p + HD) = make_float2(M, l);
-    return;
+    auto at = [&](int row) {
+      return a.part + (((int64_t)(rq.start + token_of(row)) * nh + head_of(row)) * a.parts + part) * (HD + 4);
+    };
+    rows_out(0.f, 1.f, at);
+    if (u == 0 && mine) *(float2 *)(at(r) + HD) = make_float2(M, l);
+  } else {
+    rows_out((T)0.f, l == 0.f ? 0.f : 1.f / l, [&](int row) {
+      return (T *)a.out + (int64_t)(rq.start + token_of(row)) * a.out_stride + (int64_t)head_of(row) * HD;
+    });
   }
-  T *op = (T *)a.out + (int64_t)(rq.start + mytok) * a.out_stride + (int64_t)myhead * HD;
-#pragma unroll
-  for (int i = 0; i < 16; i++)
-#pragma unroll
-    for (int e = 0; e < DT; e++) op[DT * (8 * (i / 4) + 4 * u + i % 4) + e] = (T)(l == 0.f ? 0.f : O[e][i] / l);
 }
 
 // The parts of a row joined: o = sum_p O_p 2^(M_p - M) / sum_p l_p 2^(M_p - M);

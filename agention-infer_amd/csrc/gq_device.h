@@ -65,6 +65,12 @@ __device__ __forceinline__ uint32_t ldh(const uint16_t *p) {
   return __builtin_nontemporal_load(p);
 }
 
+// N values moved together.
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
 // Dword k of an array of 16-byte chunks (k a compile-time constant after
 // unrolling, so this is a register pick).
 __device__ __forceinline__ uint32_t dw(const uint4 *ch, int k) {

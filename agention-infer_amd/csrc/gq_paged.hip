@@ -130,11 +130,6 @@ __device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return (float)v;
 template <>
 __device__ __forceinline__ float to_f32<__bf16>(__bf16 v) { return (float)v; }
 
-template <class T, int N>
-struct alignas(sizeof(T) * N) Vec {
-  T v[N];
-};
-
 // -------------------------------------------------------- rotary positions
 // Pair i of the first `rot` dims of a head (dims i, i + rot / 2 in the half
 // layout, 2 i, 2 i + 1 in the interleaved one) at position p:

@@ -68,7 +68,7 @@ class Case:
     def cache(self):
         return gq.Kv8Cache(*map(dev, self.codes), *map(dev, self.scales))
 
-    def want(self, window=0, hidden=()):
+    def want(self, window=0, most=2**31):
         """(out, tolerance) float64; NaN where a row sees a NaN."""
         q = self.q.double().cpu().numpy()
         out, tol = np.zeros(q.shape), np.zeros(q.shape)
@@ -76,7 +76,7 @@ class Case:
             ctx = self.ctx[b]
             pos = np.arange(ctx)
             ids = self.tables[b, pos // self.page] if ctx else np.zeros(0, int)
-            ok = (ids >= 0) & (ids < self.codes[0].shape[0])
+            ok = (ids >= 0) & (ids < self.codes[0].shape[0]) & (pos < most)
             ids = np.where(ok, ids, 0)
             for h in range(self.kvh):
                 k, v = (c[ids, h, pos % self.page].astype(np.float64) * s[ids, h][:, None].astype(np.float64)
@@ -165,6 +165,26 @@ def test_holes_and_empty_rows(backend, dtype):
     out = c.check(backend)
     assert (out[4:6] == 0).all() and (out[76] == 0).all()
     c.check(backend, window=20)
+
+
+@pytest.mark.parametrize("reqs", [[(100, 4), (40, 2), (9, 1)], [(100, 70), (40, 30), (9, 1)]])
+def test_bounds_hide_keys(backend, reqs):
+    """Keys past max_ctx, and past what the table holds, are not seen."""
+    for window in (0, 20):
+        for most in (25, 64, 100):
+            c = Case(reqs, 16, 2, 3, 64, "float32", seed=17)
+            got = backend.attn_kv8(c.q, c.cache(), *c.args(max_ctx=most), window=window)[:c.starts[-1]]
+            whole = c.tables.copy()
+            want, tol = c.want(window, most)
+            assert (np.abs(got.double().cpu().numpy() - want[:c.starts[-1]]) <= tol[:c.starts[-1]]).all()
+            wide = most // 16  # a table that ends there
+            c.tables = np.ascontiguousarray(whole[:, :wide])
+            got = backend.attn_kv8(c.q, c.cache(), *c.args(), window=window)[:c.starts[-1]]
+            c.tables = whole
+            want, tol = c.want(window, 16 * wide)
+            assert (np.abs(got.double().cpu().numpy() - want[:c.starts[-1]]) <= tol[:c.starts[-1]]).all()
+    c.tables = np.zeros((len(reqs), 0), np.int32)
+    assert (backend.attn_kv8(c.q, c.cache(), *c.args())[:c.starts[-1]] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
