@@ -318,6 +318,7 @@ struct AppendArgs {
   int64_t k_stride, v_stride;
   const int *slots;
   int n, heads, page, total;  // total: slots of the cache
+  int window;  // tokens that a block looks at (set by the launch)
 };
 hipError_t launch_kv8_append(const AppendArgs &a, int dtype, int hd, hipStream_t st);
 

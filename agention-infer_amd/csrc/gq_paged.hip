@@ -237,101 +237,176 @@ hipError_t launch_rope(const RopeArgs &a, int dtype, hipStream_t st) {
 // exact.  A value that is not finite makes s' NaN, and with it what the page
 // holds for that head, until rows start it anew.
 //
-// Bound by reading the rows once (twice from the L2) and writing the codes.
-// A wave takes one run: the tokens t, t + 1, ... whose slots follow each
-// other within a page.  Whether a token begins one shows from its slot and
-// the one before it.
-constexpr int APPEND_THREADS = 64;
+// Bound by reading the rows and writing the codes once.  A run is the tokens
+// t, t + 1, ... whose slots follow each other within a page; whether a token
+// begins one shows from its slot and the one before it.  A block looks for the
+// beginnings in a window of tokens (at one head of k or v): a run of up to
+// APPEND_SHORT rows is one wave's, a longer one the whole block's.  Rows stay in
+// registers between the maximum and the codes.  64 single tokens of 4 heads in
+// 4.4 us; 8184 tokens of 24 prompts, 8 bf16 heads, in 23 us (2.2 TB/s: the
+// reads of slots, rows and scales wait for one another).
+constexpr int APPEND_THREADS = 256, APPEND_WAVES = APPEND_THREADS / 64, APPEND_SHORT = 16;
 
-// rint(x / s) for finite x, |x| <= 127.5 s, rs = 1 / s (s >= 2^-60): the
-// first guess is off by less than one; the rest of the division, x - c s,
-// is exact in one fma and decides (the tie goes to the even code).
+// rint(x / s) for finite x, |x| <= 127.5 s, rs = 1 / s (s >= 2^-60).  The
+// product x rs is off by less than 127.5 * 2 * 2^-24 < 2^-15 / 2, so its
+// nearest whole number is right unless it lies that near a half (`near`); then
+// code_of decides: the rest of the division, x - c s, is exact in one fma (the
+// tie goes to the even code).
 __device__ __forceinline__ float code_of(float x, float s, float rs) {
   const float c = rintf(x * rs), rest = fmaf(-c, s, x), h = 0.5f * s;
   const float up = rest < 0.f ? -1.f : 1.f, far = fabsf(rest);
   const bool odd = ((int)c & 1) != 0;
   return far > h || (far == h && odd) ? c + up : c;
 }
+__device__ __forceinline__ float code_guess(float x, float rs, bool &near) {
+  const float y = x * rs, c = rintf(y);
+  near |= !(fabsf(y - c) <= 0.5f - 0x1p-15f);
+  return c;
+}
 
-template <class T, int HD>
-__global__ __launch_bounds__(APPEND_THREADS) void k_kv8_append(AppendArgs a) {
-  constexpr int VE = 16 / sizeof(T), LPR = HD / VE, RPI = 64 / LPR;  // lanes a row, rows an iteration
-  const int t0 = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  const bool isv = blockIdx.z;
-  const int slot = a.slots[t0];
-  if (slot < 0 || slot >= a.total) return;
+// One run of `len` rows from token t on, by W waves; `top` and `bad` of each
+// wave go through LDS.
+template <class T, int HD, int W>
+__device__ __forceinline__ void append_run(const AppendArgs &a, int t, int slot, int len, int h, bool isv, float *tops) {
+  constexpr int VE = 16 / sizeof(T), LPR = HD / VE, RPI = W * 64 / LPR;  // lanes a row, rows an iteration
+  constexpr int KEEP = LPR / 4;  // iterations whose rows stay in registers: 16 rows a wave
   const int page = slot / a.page, off = slot % a.page;
-  if (off && t0 && a.slots[t0 - 1] == slot - 1) return;  // inside a run
-  // the run's length: whole groups of 64 followers, then the first that is none
-  int len = 1;
-  const int most = min(a.page - off, a.n - t0);
-  while (len < most) {
-    const int i = len + lane;
-    const unsigned long long no = __ballot(i >= most || a.slots[t0 + i] != slot + i);
-    if (no) {
-      len += __ffsll(no) - 1;
-      break;
-    }
-    len += 64;
-  }
+  const int me = W == 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
   const int64_t stride = isv ? a.v_stride : a.k_stride;
-  const T *src = (const T *)(isv ? a.v : a.k) + t0 * stride + (int64_t)h * HD;
+  const T *src = (const T *)(isv ? a.v : a.k) + t * stride + (int64_t)h * HD;
   int8_t *codes = (isv ? a.vc : a.kc) + ((int64_t)page * a.heads + h) * a.page * HD;
   float *scale = (isv ? a.vs : a.ks) + (int64_t)page * a.heads + h;
-  const int row = lane / LPR, d = (lane % LPR) * VE;
+  const int row = me / LPR, d = (me % LPR) * VE;
   typedef Vec<T, VE> V;
+  const float old = off ? *scale : 0.f;
+  V kept[KEEP];
+#pragma unroll
+  for (int i = 0; i < KEEP; i++)
+    if (row + i * RPI < len) kept[i] = *(const V *)(src + (row + i * RPI) * stride + d);
   float top = 0.f;
   bool bad = false;
-  for (int r = row; r < len; r += RPI) {
-    const V x = *(const V *)(src + r * stride + d);
+  auto look = [&](const V &x) {
 #pragma unroll
     for (int e = 0; e < VE; e++) {
       const float f = fabsf(to_f32(x.v[e]));
       bad |= !(f <= 3.4028234663852886e38f);
       top = fmaxf(top, f);
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < KEEP; i++)
+    if (row + i * RPI < len) look(kept[i]);
+  for (int r = row + KEEP * RPI; r < len; r += RPI) look(*(const V *)(src + r * stride + d));
   top = wave_max(top);
-  bad = __any(bad);
-  const float old = off ? *scale : 0.f;
+  if (__any(bad)) top = __builtin_inff();
+  if (W > 1) {
+    if ((me & 63) == 0) tops[me / 64] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; w++) top = fmaxf(top, tops[w]);
+  }
   // (a NaN held before stays: fmaxf would drop it)
-  const float now = bad || old != old ? __builtin_nanf("") : fmaxf(fmaxf(old, top / 127.0f), KV8_MIN_SCALE);
+  const float now = top == __builtin_inff() || old != old ? __builtin_nanf("") : fmaxf(fmaxf(old, top / 127.0f), KV8_MIN_SCALE);
   if (now > old && old > 0.f) {
     const double s0 = old, s1 = now;
-    for (int i = 4 * lane; i < off * HD; i += 256) {
+    const float ratio = (float)(s0 / s1);  // (as above: |c| ratio is off by less than 2^-15 / 2)
+    for (int i = 4 * me; i < off * HD; i += W * 256) {
       const uint32_t w = *(const uint32_t *)(codes + i);
       uint32_t y = 0;
+      bool near = false;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int c = (int8_t)(w >> (8 * e));
-        y |= ((uint32_t)(int)rint((double)c * s0 / s1) & 0xffu) << (8 * e);
+      for (int e = 0; e < 4; e++)
+        y |= ((uint32_t)(int)code_guess((float)(int8_t)(w >> (8 * e)), ratio, near) & 0xffu) << (8 * e);
+      if (near) {
+        y = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          y |= ((uint32_t)(int)rint((double)(int8_t)(w >> (8 * e)) * s0 / s1) & 0xffu) << (8 * e);
       }
       *(uint32_t *)(codes + i) = y;
     }
   }
   const float rs = 1.0f / now;
-  for (int r = row; r < len; r += RPI) {
-    const V x = *(const V *)(src + r * stride + d);
-    uint32_t w[VE / 4];
+  auto put = [&](const V &x, int r) {
+    uint32_t w[VE / 4] = {};
+    bool near = false;
 #pragma unroll
-    for (int k = 0; k < VE / 4; k++) {
-      w[k] = 0;
+    for (int e = 0; e < VE; e++) w[e / 4] |= ((uint32_t)(int)code_guess(to_f32(x.v[e]), rs, near) & 0xffu) << (8 * (e & 3));
+    if (near) {  // (a NaN scale too: its codes are zeros)
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        w[k] |= ((uint32_t)(now == now ? (int)code_of(to_f32(x.v[4 * k + e]), now, rs) : 0) & 0xffu) << (8 * e);
+      for (int k = 0; k < VE / 4; k++) w[k] = 0;
+#pragma unroll
+      for (int e = 0; e < VE; e++)
+        w[e / 4] |= ((uint32_t)(now == now ? (int)code_of(to_f32(x.v[e]), now, rs) : 0) & 0xffu) << (8 * (e & 3));
     }
     int8_t *p = codes + (off + r) * HD + d;
     if constexpr (VE == 8)
       *(uint2 *)p = make_uint2(w[0], w[1]);
     else
       *(uint32_t *)p = w[0];
+  };
+#pragma unroll
+  for (int i = 0; i < KEEP; i++)
+    if (row + i * RPI < len) put(kept[i], row + i * RPI);
+  for (int r = row + KEEP * RPI; r < len; r += RPI) put(*(const V *)(src + r * stride + d), r);
+  if (me == 0) *scale = now;
+}
+
+template <class T, int HD>
+__global__ __launch_bounds__(APPEND_THREADS) void k_kv8_append(AppendArgs a) {
+  __shared__ float tops[2][APPEND_WAVES];
+  // Heads go fastest: blocks that run together read whole rows.  Runs of whole
+  // pages begin in every second, fourth, ... window, and blocks go to the CUs
+  // in turn: the windows of 32 neighbours are turned by five a group, or a
+  // quarter of the CUs would do all the work (8192 x 8 rows 72 us, not 39).
+  const int wb = blockIdx.x / a.heads, h = blockIdx.x % a.heads, lane = threadIdx.x & 63;
+  const int turned = (wb & ~31) | ((wb + 5 * (wb >> 5)) & 31);
+  const int w0 = ((wb | 31) < (int)(gridDim.x / a.heads) ? turned : wb) * a.window;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const bool isv = blockIdx.y;
+  // the window's tokens, one a lane: those that begin a run, those that go on
+  const int t = w0 + lane, wide = min(a.window, a.n - w0);
+  const int slot = lane < wide ? a.slots[t] : -1;
+  const int before = lane < wide && t ? a.slots[t - 1] : -1;
+  const bool fits = slot >= 0 && slot < a.total;
+  const bool goes_on = fits && slot % a.page && before == slot - 1;
+  const unsigned long long begins = __ballot(fits && !goes_on), other = __ballot(lane < wide && !goes_on);
+  int short_run = 0, long_run = 0;
+  for (unsigned long long left = begins; left; left &= left - 1) {
+    const int i = __ffsll(left) - 1, first = __shfl(slot, i);
+    const unsigned long long next = i < 63 ? other >> (i + 1) : 0;
+    int len;
+    if (next) {
+      len = __ffsll(next);
+    } else {  // to the window's end, then on in steps of 64
+      const int most = min(a.page - first % a.page, a.n - (w0 + i));
+      len = wide - i;
+      while (len < most) {
+        const int j = len + lane;
+        const unsigned long long no = __ballot(j >= most || a.slots[w0 + i + j] != first + j);
+        if (no) {
+          len += __ffsll(no) - 1;
+          break;
+        }
+        len += 64;
+      }
+    }
+    if (len > APPEND_SHORT)
+      append_run<T, HD, APPEND_WAVES>(a, w0 + i, first, len, h, isv, tops[long_run++ & 1]);
+    else if ((short_run++ & (APPEND_WAVES - 1)) == wave)
+      append_run<T, HD, 1>(a, w0 + i, first, len, h, isv, nullptr);
   }
-  if (lane == 0) *scale = now;
 }
 
 template <class T>
-static void append_launch(const AppendArgs &a, int hd, hipStream_t st) {
-  const dim3 g(a.n, a.heads, 2), b(APPEND_THREADS);
+static void append_launch(AppendArgs a, int hd, hipStream_t st) {
+  // Wide windows are fewer blocks; a wave takes a window's short runs one after
+  // another.  Calls of single tokens x heads in windows of 4 / 16 / 32, bf16:
+  // 256 x 8 15.0 / 19.8 / 27.4 us, 1024 x 8 27.9 / 23.2 / 28.9, 4096 x 8 72 /
+  // 54.7 / 53.6; prompts 512 x 4 17.8 / 17.5 / 17.8, 8192 x 8 55 / 39.3 / 36.6.
+  const int64_t rows = (int64_t)a.n * a.heads;
+  a.window = rows <= 4096 ? APPEND_WAVES : rows < 32768 ? 16 : 32;
+  const dim3 g((unsigned)(((int64_t)a.n + a.window - 1) / a.window * a.heads), 2), b(APPEND_THREADS);
   if (hd == 64)
     hipLaunchKernelGGL((k_kv8_append<T, 64>), g, b, 0, st, a);
   else
