@@ -112,40 +112,19 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
   const int klo = ak.lo + part * a.split, khi = (int)min((int64_t)ak.hi, (int64_t)klo + a.split);
   const int nh = a.n_kv * a.group;
 
-  // q: row m's values of this lane's dims, scaled to 2^14 .. 2^15
+  // q: row m's values of this lane's dims; on their way beside the first chunk
   const int myrow = row0 + min(m, rows - 1), mytok = myrow / a.group, myhead = kh * a.group + myrow % a.group;
   const T *qp = (const T *)a.q + (int64_t)(rq.start + mytok) * a.q_stride + (int64_t)myhead * HD + 16 * g;
-  float qv[HD / 4];
-  float qm = 0.f;
+  constexpr int VE = 16 / sizeof(T);
+  Vec<T, VE> qraw[HD / 4 / VE];
 #pragma unroll
-  for (int i = 0; i < HD / 4; i++) {
-    qv[i] = (float)qp[64 * (i / 16) + i % 16];
-    qm = fmaxf(qm, fabsf(qv[i]));
-  }
-  qm = lane_groups_max(qm);
-  int ex = 0;
-  (void)frexpf(qm, &ex);
-  const float up = qm > 0.f ? ldexpf(1.f, min(15 - ex, 126)) : 1.f;
-  const float qf = a.scale * 1.4426950408889634f / up;
-  a8_f16x8 qh[KS], ql[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float x = qv[8 * ks + j] * up;
-      qh[ks][j] = (_Float16)x;
-      if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
-    }
+  for (int i = 0; i < HD / 4 / VE; i++) qraw[i] = *(const Vec<T, VE> *)(qp + 64 * (i * VE / 16) + i * VE % 16);
   // keys that row m sees: (see_lo, see_hi]; all_lo, all_hi: that each row sees
   const int see_hi = m < rows ? min(rq.first + mytok, rq.keys - 1) : -1;
   const int see_lo = first_hidden(rq.first + mytok, a.window);
   const int all_hi = rows == 16 ? min(rq.first + row0 / a.group, rq.keys - 1) : -1;
   const int all_lo = first_hidden(rq.first + (row0 + rows - 1) / a.group, a.window);
 
-  float M = -INFINITY, l = 0.f;
-  a8_f32x4 O[DPL];
-#pragma unroll
-  for (int e = 0; e < DPL; e++) O[e] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
   const int *table = a.tables + (int64_t)b * a.wide;
 
   // The chunk at k0: `ids` its pages, K, V and scales on their way while the
@@ -190,6 +169,36 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
       }
     }
   };
+  constexpr int STEP = CHUNK * NW;
+  int k0 = klo + CHUNK * wave, ids[NT];
+  Chunk c0, c1;
+  if (k0 < khi) {
+    pages(k0, ids);
+    load(k0, ids, c0);
+    pages(k0 + STEP, ids);
+  }
+  // scaled to 2^14 .. 2^15
+  float qm = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 4; i++) qm = fmaxf(qm, fabsf((float)qraw[i / VE].v[i % VE]));
+  qm = lane_groups_max(qm);
+  int ex = 0;
+  (void)frexpf(qm, &ex);
+  const float up = qm > 0.f ? ldexpf(1.f, min(15 - ex, 126)) : 1.f;
+  const float qf = a.scale * 1.4426950408889634f / up;
+  a8_f16x8 qh[KS], ql[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float x = (float)qraw[(8 * ks + j) / VE].v[(8 * ks + j) % VE] * up;
+      qh[ks][j] = (_Float16)x;
+      if (SPLIT) ql[ks][j] = (_Float16)(x - (float)qh[ks][j]);
+    }
+  float M = -INFINITY, l = 0.f;
+  a8_f32x4 O[DPL];
+#pragma unroll
+  for (int e = 0; e < DPL; e++) O[e] = a8_f32x4{0.f, 0.f, 0.f, 0.f};
   auto work = [&](int k0, const Chunk &c) {
     float z[NT][4], ivs[NT];
 #pragma unroll
@@ -282,35 +291,25 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
       }
     }
   };
-  {
-    constexpr int STEP = CHUNK * NW;
-    int k0 = klo + CHUNK * wave, ids[NT];
-    Chunk c0, c1;
-    if (k0 < khi) {
-      pages(k0, ids);
-      load(k0, ids, c0);
-      pages(k0 + STEP, ids);
-    }
-    // (each call of work() comes behind a load that is certain, so that it
-    // waits for its own chunk's loads alone)
-    while (k0 < khi) {
-      if (k0 + STEP >= khi) {
-        work(k0, c0);
-        break;
-      }
-      load(k0 + STEP, ids, c1);
-      pages(k0 + 2 * STEP, ids);
+  // (each call of work() comes behind a load that is certain, so that it
+  // waits for its own chunk's loads alone)
+  while (k0 < khi) {
+    if (k0 + STEP >= khi) {
       work(k0, c0);
-      k0 += STEP;
-      if (k0 + STEP >= khi) {
-        work(k0, c1);
-        break;
-      }
-      load(k0 + STEP, ids, c0);
-      pages(k0 + 2 * STEP, ids);
-      work(k0, c1);
-      k0 += STEP;
+      break;
     }
+    load(k0 + STEP, ids, c1);
+    pages(k0 + 2 * STEP, ids);
+    work(k0, c0);
+    k0 += STEP;
+    if (k0 + STEP >= khi) {
+      work(k0, c1);
+      break;
+    }
+    load(k0 + STEP, ids, c0);
+    pages(k0 + 2 * STEP, ids);
+    work(k0, c1);
+    k0 += STEP;
   }
 
   // The waves' results, each to the largest M of its row.
@@ -736,15 +735,16 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
 // The parts of a row joined: o = sum_p O_p 2^(M_p - M) / sum_p l_p 2^(M_p - M);
 // rows of one part are written already.  WPR waves take a row's parts in turn
 // (1 where there are few, so that a block has 4 rows: 14336 rows of 4 parts in
-// 10 us), 4 of them at once in flight.
-constexpr int JOIN_THREADS = 256, JOIN_FEW = 8;
+// 10 us), UN of them at once in flight, each wave with the largest M that it
+// has met.
+constexpr int JOIN_FEW = 8, JOIN_WAVES = 8;
 template <class T, int HD, int WPR>
-__global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
-  constexpr int LD = HD + 4, DPL = HD / 64, UN = 4;
-  __shared__ float so[WPR][HD], sl[WPR];
+__global__ __launch_bounds__(64 * (WPR > 4 ? WPR : 4)) void k_attn_kv8_join(AttnArgs a) {
+  constexpr int LD = HD + 4, DPL = HD / 64, UN = WPR > 1 ? 8 : 4, WAVES = WPR > 4 ? WPR : 4;
+  __shared__ float so[WPR][HD], sm[WPR], sl[WPR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % WPR, kh = blockIdx.y, b = blockIdx.z;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
-  const int64_t row = (int64_t)blockIdx.x * (JOIN_THREADS / 64 / WPR) + wave / WPR;
+  const int64_t row = (int64_t)blockIdx.x * (WAVES / WPR) + wave / WPR;
   const int64_t all = (int64_t)rq.fresh * a.group;
   if (row >= all) return;
   const bool tiles = a.tparts && all > a.few;
@@ -754,26 +754,31 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
   if (n == 1) return;
   const int nh = a.n_kv * a.group, tok = rq.start + (int)(row / a.group), head = kh * a.group + (int)(row % a.group);
   const float *p = a.part + ((int64_t)tok * nh + head) * a.parts * LD;
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 64) M = fmaxf(M, p[(int64_t)i * LD + HD]);
-  M = wave_max(M);
-  float l = 0.f, o[DPL] = {};
+  float M = -INFINITY, l = 0.f, o[DPL] = {};
+  // (M_p = -inf: nothing seen, zeros; or NaN scores alone, NaN: times 1)
+  auto to = [](float m, float most) { return m == -INFINITY ? 1.f : exp2_raw(m - most); };
   for (int i0 = w; i0 < n; i0 += UN * WPR) {
     float v[UN][DPL], mi[UN], li[UN];
 #pragma unroll
     for (int j = 0; j < UN; j++) {
-      const int i = i0 + j * WPR;
-      const float *pi = p + (int64_t)min(i, n - 1) * LD;
+      const float *pi = p + (int64_t)min(i0 + j * WPR, n - 1) * LD;
       mi[j] = pi[HD];
       li[j] = pi[HD + 1];
 #pragma unroll
       for (int e = 0; e < DPL; e++) v[j][e] = pi[DPL * lane + e];
     }
+    float most = M;  // (past the last part: that one again, its M alone)
+#pragma unroll
+    for (int j = 0; j < UN; j++) most = fmaxf(most, mi[j]);
+    const float c0 = to(M, most);
+    M = most;
+    l *= c0;
+#pragma unroll
+    for (int e = 0; e < DPL; e++) o[e] *= c0;
 #pragma unroll
     for (int j = 0; j < UN; j++) {
       if (i0 + j * WPR >= n) break;
-      // (M_p = -inf: nothing seen, zeros; or NaN scores alone, NaN)
-      const float c = mi[j] == -INFINITY ? 1.f : exp2_raw(mi[j] - M);
+      const float c = to(mi[j], M);
       l = fmaf(li[j], c, l);
 #pragma unroll
       for (int e = 0; e < DPL; e++) o[e] = fmaf(v[j][e], c, o[e]);
@@ -782,14 +787,23 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_attn_kv8_join(AttnArgs a) {
   if constexpr (WPR > 1) {
 #pragma unroll
     for (int e = 0; e < DPL; e++) so[w][DPL * lane + e] = o[e];
-    if (lane == 0) sl[w] = l;
+    if (lane == 0) {
+      sm[w] = M;
+      sl[w] = l;
+    }
     __syncthreads();
     if (w) return;
 #pragma unroll
-    for (int k = 1; k < WPR; k++) {
-      l += sl[k];
+    for (int k = 0; k < WPR; k++) M = fmaxf(M, sm[k]);
+    l = 0.f;
 #pragma unroll
-      for (int e = 0; e < DPL; e++) o[e] += so[k][DPL * lane + e];
+    for (int e = 0; e < DPL; e++) o[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < WPR; k++) {
+      const float c = to(sm[k], M);
+      l = fmaf(sl[k], c, l);
+#pragma unroll
+      for (int e = 0; e < DPL; e++) o[e] = fmaf(so[k][DPL * lane + e], c, o[e]);
     }
   }
   T *op = (T *)a.out + (int64_t)tok * a.out_stride + (int64_t)head * HD + DPL * lane;
@@ -813,10 +827,10 @@ static void attn_launch(const AttnArgs &a, const AttnCut &c, hipStream_t st) {
   const int64_t all = (int64_t)a.max_new * a.group;
   const int64_t rows = c.tparts > 1 ? all : c.rparts > 1 ? std::min<int64_t>(all, c.tparts ? c.few : all) : 0;
   if (rows && c.parts > JOIN_FEW)
-    hipLaunchKernelGGL((k_attn_kv8_join<T, HD, 4>), dim3((unsigned)rows, a.n_kv, a.n_requests), dim3(JOIN_THREADS), 0, st, a);
-  else if (rows)
-    hipLaunchKernelGGL((k_attn_kv8_join<T, HD, 1>), dim3((unsigned)((rows + 3) / 4), a.n_kv, a.n_requests), dim3(JOIN_THREADS),
+    hipLaunchKernelGGL((k_attn_kv8_join<T, HD, JOIN_WAVES>), dim3((unsigned)rows, a.n_kv, a.n_requests), dim3(64 * JOIN_WAVES),
                        0, st, a);
+  else if (rows)
+    hipLaunchKernelGGL((k_attn_kv8_join<T, HD, 1>), dim3((unsigned)((rows + 3) / 4), a.n_kv, a.n_requests), dim3(256), 0, st, a);
 }
 
 hipError_t launch_attn_kv8(const AttnArgs &a, int dtype, int hd, const AttnCut &c, hipStream_t st) {

@@ -28,23 +28,33 @@ namespace gq {
 // either older than this call or recomputed from the free list, so it does not
 // matter which block writes it when.
 constexpr int PLAN_THREADS = 256;
+template <int PER>  // requests of a thread, at most
 __global__ __launch_bounds__(PLAN_THREADS) void k_page_plan(PagePlanArgs a) {
   extern __shared__ int plan_lds[];
-  int *tok0 = plan_lds, *pg0 = plan_lds + a.n + 1;
+  int *tok0 = plan_lds, *pg0 = tok0 + a.n + 1, *held0 = pg0 + a.n + 1;
   __shared__ int wsum[2][PLAN_THREADS / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // A thread's requests, all of their lengths in flight at once.
   const int per = (a.n + PLAN_THREADS - 1) / PLAN_THREADS;
-  const int i0 = min(tid * per, a.n), i1 = min(i0 + per, a.n);
-  auto before = [&](int r) { return pages_of(not_negative(a.cached[r]), a.page, a.wide); };
-  auto need = [&](int r) {
-    const int c = not_negative(a.cached[r]), all = sat_add(c, not_negative(a.fresh[r]));
-    return pages_of(all, a.page, a.wide) - pages_of(c, a.page, a.wide);
-  };
+  const int i0 = min(tid * per, a.n), mine = min(per, a.n - i0);
+  int held[PER], fresh[PER];
+#pragma unroll
+  for (int k = 0; k < PER; k++)
+    if (k < mine) {
+      held[k] = a.cached[i0 + k];
+      fresh[k] = a.fresh[i0 + k];
+    }
   int st = 0, sp = 0;
-  for (int r = i0; r < i1; r++) {
-    st = sat_add(st, not_negative(a.fresh[r]));
-    sp = sat_add(sp, need(r));
-  }
+#pragma unroll
+  for (int k = 0; k < PER; k++)
+    if (k < mine) {
+      const int c = not_negative(held[k]);
+      held0[i0 + k] = c;
+      fresh[k] = not_negative(fresh[k]);
+      held[k] = pages_of(sat_add(c, fresh[k]), a.page, a.wide) - pages_of(c, a.page, a.wide);  // its new pages
+      st = sat_add(st, fresh[k]);
+      sp = sat_add(sp, held[k]);
+    }
   int xt = st, xp = sp;  // inclusive scan over the wave
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -66,22 +76,25 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_page_plan(PagePlanArgs a) {
     et = sat_add(et, wsum[0][w]);
     ep = sat_add(ep, wsum[1][w]);
   }
-  for (int r = i0; r < i1; r++) {
-    tok0[r] = et;
-    pg0[r] = ep;
-    et = sat_add(et, not_negative(a.fresh[r]));
-    ep = sat_add(ep, need(r));
-  }
+#pragma unroll
+  for (int k = 0; k < PER; k++)
+    if (k < mine) {
+      tok0[i0 + k] = et;
+      pg0[i0 + k] = ep;
+      et = sat_add(et, fresh[k]);
+      ep = sat_add(ep, held[k]);
+    }
   if (tid == PLAN_THREADS - 1) {  // (its range ends at n)
     tok0[a.n] = et;
     pg0[a.n] = ep;
   }
   __syncthreads();
   const int tokens = tok0[a.n], pages = pg0[a.n];
+  auto before = [&](int r) { return pages_of(held0[r], a.page, a.wide); };
   if (blockIdx.x == 0) {
     for (int r = tid; r <= a.n; r += PLAN_THREADS) a.q_start[r] = tok0[r];
     for (int r = tid; r < a.n; r += PLAN_THREADS)
-      a.ctx_lens[r] = sat_add(not_negative(a.cached[r]), not_negative(a.fresh[r]));
+      a.ctx_lens[r] = sat_add(held0[r], not_negative(a.fresh[r]));
     if (tid == 0) {
       a.counts[0] = tokens;
       a.counts[1] = pages;
@@ -96,7 +109,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_page_plan(PagePlanArgs a) {
     int pos = 0, slot = -1;  // behind the last request: no slot
     if (t < tokens) {
       const int r = owner_of(tok0, a.n, (int)t);
-      pos = sat_add(not_negative(a.cached[r]), (int)t - tok0[r]);
+      pos = sat_add(held0[r], (int)t - tok0[r]);
       const int j = pos / a.page, b = before(r);
       if (j < a.wide) {
         int id = -1;
@@ -116,7 +129,11 @@ hipError_t launch_page_plan(const PagePlanArgs &a, hipStream_t st) {
   const int work = a.max_tokens > a.n ? a.max_tokens : a.n;
   int blocks = (work + PLAN_THREADS - 1) / PLAN_THREADS;
   blocks = blocks < 1 ? 1 : blocks > 512 ? 512 : blocks;
-  hipLaunchKernelGGL(k_page_plan, dim3(blocks), dim3(PLAN_THREADS), 2 * (size_t)(a.n + 1) * sizeof(int), st, a);
+  const size_t lds = (3 * (size_t)a.n + 2) * sizeof(int);
+  if (a.n <= 2 * PLAN_THREADS)
+    hipLaunchKernelGGL(k_page_plan<2>, dim3(blocks), dim3(PLAN_THREADS), lds, st, a);
+  else
+    hipLaunchKernelGGL(k_page_plan<PAGE_PLAN_MAX_REQUESTS / PLAN_THREADS>, dim3(blocks), dim3(PLAN_THREADS), lds, st, a);
   return hipGetLastError();
 }
 
