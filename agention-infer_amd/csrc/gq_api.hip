@@ -1081,6 +1081,8 @@ int check_kv8(const gq_kv8 *c) {
   if (c->n_kv_heads < 1 || c->n_kv_heads > 65535) return fail(GQ_EINVAL, "%d KV heads", c->n_kv_heads);
   if (c->n_pages < 1 || (int64_t)c->n_pages * c->page_size > INT_MAX)
     return fail(GQ_EINVAL, "%d pages of %d tokens: 1 to 2^31 - 1 slots are needed", c->n_pages, c->page_size);
+  if ((int64_t)c->n_pages * c->n_kv_heads > INT_MAX)
+    return fail(GQ_EINVAL, "%d pages of %d KV heads: at most 2^31 - 1 scales are possible", c->n_pages, c->n_kv_heads);
   if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(GQ_EINVAL, "null cache buffer");
   if (!aligned16(c->k) || !aligned16(c->v)) return fail(GQ_EINVAL, "cache codes must start at a multiple of 16 bytes");
   return GQ_OK;
@@ -1172,9 +1174,9 @@ int gq_rope(int dtype, int layout, int n, int head_dim, int rot_dim, const doubl
   if (int rc = check_type("gq_rope", dtype)) return rc;
   if (layout != GQ_ROPE_HALF && layout != GQ_ROPE_INTERLEAVED) return fail(GQ_EINVAL, "unknown RoPE layout %d", layout);
   if (!k_dev) n_kv_heads = 0, k_stride = k_out_stride = 0, k_out_dev = nullptr;
-  if (n < 0 || n_heads < 1 || n_kv_heads < 0 || n_heads > 65535 || n_kv_heads > 65535 || head_dim < 2 || head_dim > 4096 ||
+  if (n < 0 || n >= 1 << 24 || n_heads < 1 || n_kv_heads < 0 || n_heads > 65535 || n_kv_heads > 65535 || head_dim < 2 || head_dim > 4096 ||
       rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim)
-    return fail(GQ_EINVAL, "gq_rope: %d tokens, %d and %d heads of %d (at most 4096), %d of them turned (even)", n, n_heads,
+    return fail(GQ_EINVAL, "gq_rope: %d tokens (less than 2^24), %d and %d heads of %d (at most 4096), %d of them turned (even)", n, n_heads,
                 n_kv_heads, head_dim, rot_dim);
   if (n == 0) return GQ_OK;
   if (!inv_freq_dev || !pos_dev || !q_dev || !q_out_dev || (k_dev && !k_out_dev)) return fail(GQ_EINVAL, "gq_rope: null buffer");
@@ -1196,6 +1198,8 @@ int gq_kv8_append(const gq_kv8 *c, int dtype, const void *k_dev, int64_t k_strid
   if (int rc = check_type("gq_kv8_append", dtype)) return rc;
   if (n < 0) return fail(GQ_EINVAL, "negative token count %d", n);
   if (n == 0) return GQ_OK;
+  if ((int64_t)n * c->n_kv_heads >= 1 << 28)  // (a grid has less than 2^32 threads)
+    return fail(GQ_EINVAL, "gq_kv8_append: %d tokens of %d heads in one call", n, c->n_kv_heads);
   const int64_t w = (int64_t)c->n_kv_heads * c->head_dim;
   if (int rc = check_rows("k", k_dev, k_stride, w, dtype)) return rc;
   if (int rc = check_rows("v", v_dev, v_stride, w, dtype)) return rc;
@@ -1211,7 +1215,7 @@ int gq_kv8_read(const gq_kv8 *c, const int *slots_dev, int n, int dtype, void *k
   if (int rc = check_kv8(c)) return rc;
   if (int rc = check_type("gq_kv8_read", dtype)) return rc;
   const int64_t w = (int64_t)c->n_kv_heads * c->head_dim;
-  if (n < 0 || n * w / 1024 > INT_MAX) return fail(GQ_EINVAL, "gq_kv8_read: %d tokens in one call", n);
+  if (n < 0 || n * w / 1024 >= (1 << 24) - 1) return fail(GQ_EINVAL, "gq_kv8_read: %d tokens in one call", n);
   if (n == 0 || (!k_out_dev && !v_out_dev)) return GQ_OK;
   for (const void *p : {k_out_dev, v_out_dev})
     if (p)
@@ -1234,7 +1238,7 @@ int check_attn(const gq_kv8 *c, int n_heads, int n_tokens, int n_requests, int m
       max_ctx > 1 << 30)
     return fail(GQ_EINVAL, "gq_attn_kv8: %d tokens, %d requests (at most 65535), max_new %d, max_ctx %d (at most 2^30)", n_tokens,
                 n_requests, max_new, max_ctx);
-  if ((int64_t)max_new * (n_heads / c->n_kv_heads) > INT_MAX - 64)
+  if ((int64_t)max_new * (n_heads / c->n_kv_heads) >= 1 << 23)  // (a join's threads)
     return fail(GQ_EINVAL, "gq_attn_kv8: max_new %d of %d heads: too many rows", max_new, n_heads);
   return GQ_OK;
 }
@@ -1266,8 +1270,8 @@ int gq_attn_kv8(const gq_kv8 *c, int dtype, const void *q_dev, int64_t q_stride,
   if (need && (!workspace_dev || workspace_bytes < need))
     return fail(GQ_ESHORT, "gq_attn_kv8: workspace: need %zu bytes, have %zu", need, workspace_dev ? workspace_bytes : 0);
   if (!aligned16(workspace_dev)) return fail(GQ_EINVAL, "gq_attn_kv8: the workspace must start at a multiple of 16 bytes");
-  const int64_t of = (int64_t)c->n_kv_heads * n_requests;  // (a grid's blocks)
-  if (cut.rtiles * cut.rparts > INT_MAX / of || cut.ttiles * cut.tparts > INT_MAX / of)
+  const int64_t of = (int64_t)c->n_kv_heads * n_requests;  // (a grid has less than 2^32 threads)
+  if (cut.rtiles * cut.rparts > ((1 << 24) - 1) / of || cut.ttiles * cut.tparts > ((1 << 23) - 1) / of)
     return fail(GQ_EINVAL, "gq_attn_kv8: too many rows by keys in one call");
   if (int rc = ensure_init()) return rc;
   const gq::AttnArgs a{c->k,       c->v,         c->k_scale,    c->v_scale,    q_dev,      out_dev,        q_stride, out_stride,

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
   const int of = a.n_kv * a.n_requests, i0 = blockIdx.x % of, step = blockIdx.x / of;
   const int kh = i0 % a.n_kv, b = i0 / a.n_kv, tile = step % a.rtiles, part = step / a.rtiles;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
-  const int64_t all = (int64_t)rq.fresh * a.group;
+  const int64_t all = (int64_t)min(rq.fresh, a.max_new) * a.group;
   if (a.tparts && all > a.few) return;  // k_attn_kv8_tiles has them
   const int rows = min(all - (int64_t)tile * 16, (int64_t)16);
   if (rows <= 0) return;
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
   const int kh = blockIdx.x % a.n_kv, bx = blockIdx.x / a.n_kv, step = bx % (a.ttiles * a.tparts);
   const int b = bx / (a.ttiles * a.tparts), tile = a.ttiles - 1 - step / a.tparts, part = step % a.tparts;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
-  const int64_t all = (int64_t)rq.fresh * a.group;
+  const int64_t all = (int64_t)min(rq.fresh, a.max_new) * a.group;
   if (all <= a.few || (int64_t)tile * TILE_ROWS >= all) return;
   const int row0 = tile * TILE_ROWS, rows = (int)min(all - row0, (int64_t)TILE_ROWS);
   const AttnKeys ak = attn_keys(rq, row0 / a.group, (row0 + rows - 1) / a.group, a.window);
@@ -745,7 +745,7 @@ __global__ __launch_bounds__(64 * (WPR > 4 ? WPR : 4)) void k_attn_kv8_join(Attn
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % WPR, kh = blockIdx.y, b = blockIdx.z;
   const AttnRequest rq = attn_request(a.q_start[b], a.q_start[b + 1], a.ctx_lens[b], a.n_tokens, a.wide, a.page, a.max_ctx);
   const int64_t row = (int64_t)blockIdx.x * (WAVES / WPR) + wave / WPR;
-  const int64_t all = (int64_t)rq.fresh * a.group;
+  const int64_t all = (int64_t)min(rq.fresh, a.max_new) * a.group;
   if (row >= all) return;
   const bool tiles = a.tparts && all > a.few;
   const int height = tiles ? TILE_ROWS : 16, row0 = (int)(row / height * height);  // of its tile

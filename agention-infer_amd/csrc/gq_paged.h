@@ -96,7 +96,7 @@ GQ_HD int attn_parts(const AttnKeys &k, int split) {
 // parts of `split`; the others (tparts 0: there are none) tiles of
 // ATTN_TILE_ROWS, ttiles at most, with parts of `tsplit`.  Parts fill the GPU
 // where there are few tiles, and even out requests of different lengths.
-constexpr int ATTN_FEW_ROWS = 64, ATTN_TILE_ROWS = 256;
+constexpr int ATTN_FEW_ROWS = 64, ATTN_TILE_ROWS = 256, ATTN_MANY_BLOCKS = 65536;
 struct AttnCut {
   int64_t rtiles, ttiles;
   int few;
@@ -121,7 +121,10 @@ inline AttnCut attn_cut(int n_tokens, int n_requests, int n_kv_heads, int group,
   if (c.rtiles) {
     // two blocks a CU at least; with enough work parts of 1024 keys (4 chunks
     // a wave) or so
-    const int64_t blocks = heads ? heads * c.rtiles : 1, k = ((int64_t)max_ctx + 1023) / 1024;
+    const int64_t blocks = heads ? heads * c.rtiles : 1;
+    int64_t k = ((int64_t)max_ctx + 1023) / 1024;
+    // (a bound on the workspace: where blocks are many, parts even out little)
+    if (blocks * k > ATTN_MANY_BLOCKS) k = ATTN_MANY_BLOCKS / blocks;
     attn_split(blocks * k >= 512 ? k : (512 + blocks - 1) / blocks, max_ctx, c.split, c.rparts);
     c.parts = c.rparts;
   }

@@ -266,7 +266,7 @@ int gq_model_generate(gq_model *m, int token, int pos, int n_steps, int *tokens_
  * The cache: n_pages pages of page_size tokens (a multiple of 16, at most
  * 256), head_dim 64 or 128.  A value is code * scale, codes -127 .. 127, one
  * f32 scale for each page and KV head.  Slot s is offset s % page_size of page
- * s / page_size; n_pages * page_size < 2^31.  Code buffers start at multiples
+ * s / page_size; n_pages * page_size < 2^31, n_pages * n_kv_heads < 2^31.  Code buffers start at multiples
  * of 16 bytes.  The caller owns the buffers; they need no initialisation. */
 typedef struct {
   int n_pages, page_size, n_kv_heads, head_dim;
@@ -326,7 +326,7 @@ int gq_rope_freqs(const gq_rope_desc *d, double *inv_freq_host, float *mscale);
  * head in pairs (i, i + rot_dim / 2) (GQ_ROPE_HALF) or (2 i, 2 i + 1)
  * (GQ_ROPE_INTERLEAVED), pair i turned by pos * inv_freq[i], times mscale; the
  * others as they are.  The angle is exact to 64 bits, at any position.  An
- * output is its input's buffer (same stride) or overlaps nothing. */
+ * output is its input's buffer (same stride) or overlaps nothing.  n < 2^24. */
 #define GQ_ROPE_HALF 0
 #define GQ_ROPE_INTERLEAVED 1
 int gq_rope(int dtype, int layout, int n, int head_dim, int rot_dim, const double *inv_freq_dev, float mscale,
@@ -347,7 +347,7 @@ int gq_rope(int dtype, int layout, int n, int head_dim, int rot_dim, const doubl
  * The rows that a call writes into a page are neighbours in the call, in the
  * order of their slots (gq_page_plan's are); what a page holds after a call
  * that breaks this is not specified.  Buffers and strides are multiples of 16
- * bytes. */
+ * bytes; n * n_kv_heads < 2^28. */
 int gq_kv8_append(const gq_kv8 *cache, int dtype, const void *k_dev, int64_t k_stride, const void *v_dev,
                   int64_t v_stride, const int *slots_dev, int n, void *stream);
 
@@ -368,12 +368,12 @@ int gq_kv8_read(const gq_kv8 *cache, const int *slots_dev, int n, int dtype, voi
  * effect on it, whatever they hold.  out has q's type; sums and the softmax
  * are f32, products carry 22 bits of f32 q and of the weights (11 for 16-bit
  * types).  The cache's scales are as gq_kv8_append leaves them (>= 2^-60).
- * max_new and max_ctx bound the rows and positions of a request: rows past
- * max_new are not computed, keys past max_ctx (or the table) not seen.  Rows
- * that belong to no request, behind q_start[n_requests] among them, are left
- * as they are.  At most 65535 requests, max_ctx at most 2^30; a new row's own k and v are in the
- * cache before the call.  Buffers and strides are multiples of 16 bytes; out
- * overlaps nothing.
+ * max_new and max_ctx bound the rows and positions of a request: keys past
+ * max_ctx (or the table) are not seen, rows past max_new, and those that belong
+ * to no request, behind q_start[n_requests] among them, are left as they are.
+ * At most 65535 requests, max_ctx at most 2^30, max_new * n_heads / n_kv_heads
+ * less than 2^23; a new row's own k and v are in the cache before the call.
+ * Buffers and strides are multiples of 16 bytes; out overlaps nothing.
  * The workspace is the caller's: gq_attn_kv8_workspace bytes (0 where none is
  * needed or the sizes are refused) at a multiple of 16, for one call at a time
  * (captured calls that are replayed side by side need their own). */

@@ -187,6 +187,21 @@ def test_bounds_hide_keys(backend, reqs):
     assert (backend.attn_kv8(c.q, c.cache(), *c.args())[:c.starts[-1]] == 0).all()
 
 
+@pytest.mark.parametrize("reqs,most", [([(2000, 12), (30, 3)], 5), ([(0, 70), (700, 90), (9, 1)], 33), ([(10, 300)], 43)])
+def test_rows_past_max_new_stay(backend, reqs, most):
+    """Rows within max_new are the request's own, the others left alone: in
+    the same tile, with and without parts."""
+    import torch
+    c = Case(reqs, 16, 2, 3, 64, "float32", seed=18)
+    out = torch.full(c.q.shape, 7.5, dtype=c.t, device="cuda")
+    backend.attn_kv8(c.q, c.cache(), *c.args(max_new=most), out=out)
+    want, tol = c.want()
+    got = out.double().cpu().numpy()
+    for b, m in enumerate(c.new):
+        s = c.starts[b]
+        assert (np.abs(got - want) <= tol)[s:s + min(m, most)].all() and (got[s + most:s + m] == 7.5).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reqs", [[(100, 2), (90, 2)], [(100, 80), (3, 2)]])
 def test_not_finite_pages(backend, dtype, reqs):

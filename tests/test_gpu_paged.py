@@ -316,6 +316,32 @@ def test_append_and_read(backend, dtype, page, heads, hd):
             assert (np.abs(got - want)[~np.isnan(want)] <= tol[~np.isnan(want)]).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,hd,page,lengths", [
+    (3, 64, 16, [1] * 900 + [5] * 90),              # single tokens, drafts
+    (8, 128, 64, [700, 1, 64, 1, 2, 129, 300, 17] + [1] * 40),
+    (8, 64, 256, [1500, 255, 257, 1, 2000, 31, 33]),
+    (16, 64, 48, [1, 2, 3, 16, 17, 18, 47, 48, 49] * 11)])
+def test_append_many(backend, dtype, heads, hd, page, lengths):
+    """Passes of hundreds and thousands of rows: runs of every length that
+    begin anywhere, twice, the second time behind the first."""
+    import torch
+    say(f"append {dtype} heads={heads} page={page} rows={sum(lengths)}")
+    t = getattr(torch, dtype)
+    rng = np.random.default_rng(heads + page)
+    need = [-(-2 * m // page) for m in lengths]
+    n_pages = sum(need)
+    ref = RefCache(n_pages, page, heads, hd, rng)
+    cache = ref.on_gpu()
+    ids, first = rng.permutation(n_pages), np.concatenate([[0], np.cumsum(need)])
+    for turn in range(2):
+        slots = [int(ids[first[r] + p // page]) * page + p % page for r, m in enumerate(lengths) for p in range(turn * m, turn * m + m)]
+        x, vals = rows_of(rng, len(slots), heads, hd, t, np.float32(1 + turn))
+        ref.append(vals, slots)
+        backend.kv8_append(cache, x[0], x[1], i32(slots))
+        same_cache(cache, ref)
+
+
 def test_append_ties_and_ranges(backend):
     """Quotients at, just below and just above a half; values so small that
     the smallest scale holds; the largest finite ones; zeros."""

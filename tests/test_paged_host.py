@@ -46,7 +46,7 @@ ROPE = dict(dtype=gq.F32, layout=0, n=2, hd=64, rot=64, freq=P, mscale=1.0, pos=
 
 @pytest.mark.parametrize("change,code,text", [
     (dict(dtype=12), EDTYPE, "Q4_K"), (dict(dtype=7), EDTYPE, "unknown"), (dict(layout=2), EINVAL, "layout 2"),
-    (dict(n=-1), EINVAL, "-1 tokens"), (dict(rot=63), EINVAL, "63 of them"), (dict(rot=66), EINVAL, "66 of them"),
+    (dict(n=-1), EINVAL, "-1 tokens"), (dict(n=1 << 24), EINVAL, "less than 2^24"), (dict(rot=63), EINVAL, "63 of them"), (dict(rot=66), EINVAL, "66 of them"),
     (dict(rot=0), EINVAL, "0 of them"), (dict(hd=4098), EINVAL, "heads of 4098"), (dict(nq=0), EINVAL, "0 and 1 heads"),
     (dict(qs=127), EINVAL, "stride"), (dict(qos=127), EINVAL, "stride"), (dict(ks=63), EINVAL, "stride"),
     (dict(kos=0), EINVAL, "stride"), (dict(q=None), EINVAL, "null"), (dict(qo=None), EINVAL, "null"),
@@ -67,7 +67,7 @@ def test_no_tokens_are_no_work():
 
 CACHES = [(dict(page=20), "page_size 20"), (dict(page=512), "page_size 512"), (dict(hd=96), "head_dim 96"),
           (dict(heads=0), "0 KV heads"), (dict(heads=65536), "65536 KV heads"), (dict(n_pages=0), "0 pages"),
-          (dict(n_pages=1 << 27), "slots"), (dict(k=None), "null cache"), (dict(v=None), "null cache"),
+          (dict(n_pages=1 << 27), "slots"), (dict(n_pages=1 << 20, heads=2048), "scales"), (dict(k=None), "null cache"), (dict(v=None), "null cache"),
           (dict(ks=None), "null cache"), (dict(vs=None), "null cache"), (dict(k=P + 8), "multiple of 16"),
           (dict(v=P + 4), "multiple of 16")]
 
@@ -91,7 +91,8 @@ ATTN = dict(dtype=gq.F32, q=P, qs=256, nh=4, n=8, tables=P, wide=4, q_start=P, c
     (dict(max_new=-1), EINVAL, "max_new -1"), (dict(max_ctx=-1), EINVAL, "max_ctx -1"),
     (dict(max_ctx=2**30 + 1), EINVAL, "at most 2"), (dict(wide=-1), EINVAL, "max_pages -1"),
     (dict(window=-1), EINVAL, "window -1"), (dict(scale=math.inf), EINVAL, "scale"), (dict(scale=math.nan), EINVAL, "scale"),
-    (dict(max_new=2**30), EINVAL, "too many rows"), (dict(qs=255), EINVAL, "q: rows"), (dict(os=128), EINVAL, "out: rows"),
+    (dict(max_new=2**30), EINVAL, "too many rows"), (dict(max_new=2**22), EINVAL, "too many rows"),
+    (dict(nr=65535, max_new=2**20), EINVAL, "by keys"), (dict(qs=255), EINVAL, "q: rows"), (dict(os=128), EINVAL, "out: rows"),
     (dict(qs=257), EINVAL, "multiples of 16"), (dict(os=258), EINVAL, "multiples of 16"), (dict(q=P + 4), EINVAL, "multiples of 16"),
     (dict(out=P + 8), EINVAL, "multiples of 16"), (dict(q=None), EINVAL, "null q"), (dict(out=None), EINVAL, "null out"),
     (dict(tables=None), EINVAL, "null"), (dict(q_start=None), EINVAL, "null"), (dict(ctx=None), EINVAL, "null"),
@@ -107,7 +108,7 @@ def test_attention_refuses(change, code, text):
     (gq.BF16, P, 132, P, 128, P, 2, EINVAL, "multiples of 16"), (gq.F32, P + 4, 128, P, 128, P, 2, EINVAL, "multiples of 16"),
     (gq.F16, P, 128, P + 8, 128, P, 2, EINVAL, "multiples of 16"), (gq.F32, None, 128, P, 128, P, 2, EINVAL, "null k"),
     (gq.F32, P, 128, None, 128, P, 2, EINVAL, "null v"), (gq.F32, P, 128, P, 128, None, 2, EINVAL, "null slots"),
-    (gq.F32, P, 128, P, 128, P, -1, EINVAL, "negative")])
+    (gq.F32, P, 128, P, 128, P, -1, EINVAL, "negative"), (gq.F32, P, 128, P, 128, P, 1 << 27, EINVAL, "in one call")])
 def test_append_refuses(dtype, k, ks, v, vs, slots, n, code, text):
     refused(gq.lib().gq_kv8_append(kv8(), dtype, k, ks, v, vs, slots, n, None), code, text)
 
@@ -118,6 +119,7 @@ def test_read_refuses():
     refused(gq.lib().gq_kv8_read(kv8(), None, 2, gq.F32, P, P, None), EINVAL, "null slots")
     refused(gq.lib().gq_kv8_read(kv8(), P, 2, gq.F32, P + 4, P, None), EINVAL, "multiples of 16")
     refused(gq.lib().gq_kv8_read(kv8(heads=65535, hd=128, n_pages=1), P, 1 << 30, gq.F32, P, P, None), EINVAL, "in one call")
+    refused(gq.lib().gq_kv8_read(kv8(heads=2, hd=64), P, 1 << 27, gq.F32, P, P, None), EINVAL, "in one call")
 
 
 # ------------------------------------------------------ rotary frequencies
@@ -277,3 +279,6 @@ def test_attention_cut(ask):
         else:
             assert ttiles == tparts == 0
         assert parts == max(rparts, tparts)
+        if few and c <= 2**30:  # and what parts add to the workspace and the grid is bounded
+            blocks = r * kv * rtiles
+            assert rparts <= max(1, 65536 // blocks, -(-512 // blocks))
