@@ -281,4 +281,4 @@ def test_attention_cut(ask):
         assert parts == max(rparts, tparts)
         if few and c <= 2**30:  # and what parts add to the workspace and the grid is bounded
             blocks = r * kv * rtiles
-            assert rparts <= max(1, 65536 // blocks, -(-512 // blocks))
+            assert rparts <= max(1, 8192 // blocks, -(-512 // blocks))
