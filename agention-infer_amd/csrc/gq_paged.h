@@ -119,10 +119,11 @@ inline AttnCut attn_cut(int n_tokens, int n_requests, int n_kv_heads, int group,
   const int64_t few = rows < c.few ? rows : c.few;
   c.rtiles = (few + 15) / 16;
   if (c.rtiles) {
-    // two blocks a CU at least; with enough work parts of 1024 keys (4 chunks
-    // a wave) or so
+    // two blocks a CU at least; with enough work parts of 1536 keys (of 512 / 768 /
+    // 1024 / 1536 / 2048 / 4096: 64 requests of 127 .. 8191 keys 136 / 127 / 122 / 118 /
+    // 118 / 124 us, 32 of 100 .. 8192 - / - / 84 / 84 / 91 / 90 us)
     const int64_t blocks = heads ? heads * c.rtiles : 1;
-    int64_t k = ((int64_t)max_ctx + 1023) / 1024;
+    int64_t k = ((int64_t)max_ctx + 1535) / 1536;
     // (with many blocks longer parts cost less, and bound the workspace: up to 2^22 /
     // 65536 / 16384 / 8192 blocks, 256 requests of 100 .. 8192 keys in 489 / 484 / 490 /
     // 456 us, 1024 of 100 .. 16384 in 3.54 / 3.11 / 2.91 / 2.93 ms)
