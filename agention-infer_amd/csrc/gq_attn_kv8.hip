@@ -74,6 +74,9 @@ __device__ __forceinline__ int first_hidden(int pos, int window) {
 // A block is one tile of 16 query rows of a (request, KV head) over one part
 // of its keys.  Rows are the request's tokens by the KV head's query heads, so
 // the heads that share K and V, and a draft's tokens, share one read of them.
+// Bound by that read: 1024 requests of 16000 .. 16384 keys, 8 bf16 KV heads of 128,
+// at 6.2 TB/s; 64 of 127 .. 8191, 547 MB, with the start and the ragged end in
+// 111 us.
 // Its 4 waves take chunks of 32 keys in turn, each with its own M, l, O, and
 // meet once at the end; nothing goes through LDS before that:
 //   S^T = K . q^T  A = 16 keys x 32 dims.  Lane (m = lane % 16, g = lane / 16)
@@ -370,8 +373,16 @@ __global__ __launch_bounds__(ROWS_THREADS, 2) void k_attn_kv8_rows(AttnArgs a) {
 // half (O of the last chunk, S of this one, and between those instructions the
 // conversion of the chunk after next and the loads of the one behind it) and a
 // vector half (softmax), and the halves of the block are one of them apart, so
-// that one wave's matrix instructions run beside the other's exponentials.  So
-// K lives in 3 buffers and V in 4: chunk n + 2 is written while n - 1 .. n + 1 are read.
+// that one wave's matrix instructions run beside the other's exponentials; the
+// matrix half issues first (8192 tokens from position 0, 32 bf16 heads of 128 over
+// 8: 630 -> 605 us, heads of 64 459 -> 425).  So K lives in 3 buffers and V in 4:
+// chunk n + 2 is written while n - 1 .. n + 1 are read.
+//
+// Bound by the matrix half: 32 instructions, 1024 cycles, take about 2000 with
+// the chunk's 32 LDS reads a wave and the staging between them (bf16; the softmax
+// half takes 1550), at the 1.9 GHz that the card keeps under this load.  That case
+// runs at 907 TFLOP/s, f32 (twice the products) at 570; a large bf16 product of
+// the library at 1210.  The staging in the vector half instead: 660 us.
 constexpr int TILE_ROWS = ATTN_TILE_ROWS, TILE_THREADS = 512;
 typedef float a8_f32x16 __attribute__((ext_vector_type(16)));
 
@@ -671,11 +682,13 @@ __global__ __launch_bounds__(TILE_THREADS, 2) void k_attn_kv8_tiles(AttnArgs a) 
     }
   } else {
     for (int n = 0; n < chunks; n++) {
+      __builtin_amdgcn_s_setprio(1);
       pv((vb + VB - 1) & (VB - 1));
       qk(kb);
       store(raw, kb ? kb - 1 : KB - 1, vb ^ 2);  // (kb + 2) % 3, (vb + 2) % 4
       load(raw);
       order();
+      __builtin_amdgcn_s_setprio(0);
       __syncthreads();
       softmax(klo + 64 * n, vb);
       __syncthreads();
