@@ -10,8 +10,9 @@ E_s + 2^-11 + 2^-20; numerator and denominator each carry that once, and the sum
 of N products in f32 adds (N / 32 + 64) 2^-24.  Together, per value,
   (2 E_s + 2^-18 (+ 2^-11 for 16-bit types) + (N / 32 + 64) 2^-24) sum p|v| + half a step of |o|.
 Small weights: a weight times its page's V scale is held as f16, the largest
-at 2^15, and f16 has no steps below 2^-24, so each is also off by up to 2^-25 /
-2^15 of the largest: 2^-40 max(p vs) sum|code|, twice that in two parts.
+of a row between 2^14 and 2^15.9, and f16 has no steps below 2^-24, so each (its
+last part, where there are two) is also off by up to 2^-25 / 2^14 of the largest:
+2^-39 max(p vs) sum|code|.
 """
 import numpy as np
 import pytest
