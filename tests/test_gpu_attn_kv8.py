@@ -411,6 +411,78 @@ def test_whole_pass(backend):
         cached = ctx
 
 
+def test_captured_pass(backend):
+    """Plan, rotary positions, append and attention captured once, with room
+    for 40 rows, replayed for passes of other lengths (padded, empty, a
+    request that ends): the same bits as eager passes of exact size, in
+    outputs and cache."""
+    import torch
+    rng = np.random.default_rng(19)
+    page, kvh, group, hd, nr, room, most, bound = 16, 2, 3, 64, 4, 40, 20, 120
+    nh = kvh * group
+    inv, m = gq.rope_freqs(hd, 1e4)
+    inv = dev(inv)
+    order = rng.permutation(32).astype(np.int32)
+
+    class Side:
+        def __init__(self):
+            self.cache = gq.kv8_cache(32, page, kvh, hd)
+            for t in self.cache:
+                t.zero_()
+            self.tables = torch.full((nr, 8), -1, dtype=torch.int32, device="cuda")
+            self.free, self.cached, self.new = i32(order), i32([0] * nr), i32([1] * nr)
+
+        def run(self, q, k, v, rows):
+            plan = backend.page_plan(self.cached, self.new, page, self.free, self.tables, rows)
+            qr, kr = backend.rope(q, k, plan.positions, inv, mscale=m)
+            backend.kv8_append(self.cache, kr, v, plan.slots)
+            out = torch.full_like(q, 7.5)
+            return plan, backend.attn_kv8(qr, self.cache, self.tables, plan.q_start, plan.ctx_lens, most, bound, out=out)
+
+    a, b = Side(), Side()
+    q, k, v = (torch.zeros((room, h, hd), device="cuda") for h in (nh, kvh, kvh))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plan, out = a.run(q, k, v, room)
+    cached, taken = np.zeros(nr, int), 0
+    for new in ([20, 3, 0, 15], [1, 1, 1, 1], [0, 17, 20, 0], [0, 0, 0, 0], [1, 0, 1, 12], [1, 1, 1, 1]):
+        n = sum(new)
+        for t in (q, k, v):
+            t.copy_(dev(rng.standard_normal(tuple(t.shape), np.float32)))
+        for side in (a, b):
+            side.cached.copy_(i32(cached))
+            side.new.copy_(i32(new))
+            side.free.copy_(i32(np.roll(order, -taken)))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        exact, want = b.run(q[:n].contiguous(), k[:n].contiguous(), v[:n].contiguous(), n)
+        assert torch.equal(out[:n], want) and (out[n:] == 7.5).all() and (plan.slots[n:] == -1).all()
+        assert torch.equal(plan.slots[:n], exact.slots) and torch.equal(a.tables, b.tables)
+        for x, y in zip(a.cache, b.cache):
+            assert torch.equal(x, y)
+        cached += new
+        taken += int(exact.counts[1])
+        float(want.sum())
+
+
+def test_most_requests(backend):
+    """65535 requests of one token that see one key, or none: its values."""
+    import torch
+    n, kvh, hd, page = 65535, 2, 64, 16
+    cache = gq.kv8_cache(4, page, kvh, hd)
+    x = [torch.randn((4, kvh, hd), device="cuda") for _ in "kv"]
+    backend.kv8_append(cache, *x, i32([0, 16, 32, 48]))
+    ids = torch.arange(n, device="cuda") % 5  # 4: not a page of the cache
+    v = backend.kv8_read(cache, i32([0, 16, 32, 48, -1]))[1]
+    out = backend.attn_kv8(torch.randn((n, 2 * kvh, hd), device="cuda"), cache, ids.int().view(n, 1), i32(np.arange(n + 1)),
+                           torch.ones(n, dtype=torch.int32, device="cuda"), 1, 1)
+    want = v[ids].repeat_interleave(2, 1)
+    # one weight w: w c / (w / vs), with exp2's, the parts' and the reciprocal's roundings
+    assert ((out - want).abs() <= 2.0**-18 * want.abs()).all() and (out[ids == 4] == 0).all()
+
+
 def test_refuses_tensors(backend):
     import torch
     c = Case([(20, 2), (3, 1)], 16, 2, 2, 64, "float32")

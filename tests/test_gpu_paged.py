@@ -219,7 +219,7 @@ def test_rope_refuses_tensors(backend):
     pos, f = i32([0, 1]), dev(gq.rope_freqs(64)[0])
     for bad in (dict(q=q.double()), dict(q=q[0]), dict(q=q.transpose(1, 2)), dict(k=k.half()), dict(k=k[:1]),
                 dict(k=k[..., :32]), dict(positions=pos.long()), dict(positions=pos[:1]), dict(positions=pos.cpu()),
-                dict(inv_freq=f.float()), dict(inv_freq=f.cpu()), dict(layout="neox"), dict(q_out=q[:1]), dict(k_out=q),
+                dict(inv_freq=f.float()), dict(inv_freq=f.cpu()), dict(layout="whole"), dict(q_out=q[:1]), dict(k_out=q),
                 dict(q=q[:1].expand(2, 4, 64))):
         with pytest.raises((ValueError, gq.GqError)):
             backend.rope(**{**dict(q=q, k=k, positions=pos, inv_freq=f), **bad})
