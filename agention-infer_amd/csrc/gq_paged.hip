@@ -264,21 +264,47 @@ hipError_t launch_rope(const RopeArgs &a, int dtype, hipStream_t st) {
 // reads of slots, rows and scales wait for one another).
 constexpr int APPEND_THREADS = 256, APPEND_WAVES = APPEND_THREADS / 64, APPEND_SHORT = 16;
 
-// rint(x / s) for finite x, |x| <= 127.5 s, rs = 1 / s (s >= 2^-60).  The
-// product x rs is off by less than 127.5 * 2 * 2^-24 < 2^-15 / 2, so its
-// nearest whole number is right unless it lies that near a half (`near`); then
-// code_of decides: the rest of the division, x - c s, is exact in one fma (the
-// tie goes to the even code).
+// rint(x / s) for finite x, |x| <= 127.5 s, rs = 1 / s (s >= 2^-60).  x rs is off
+// from the quotient by less than 127.5 * 2^-24, so its nearest whole number is
+// right unless it lies within 2^-15 of a half; then code_of decides: the rest of
+// the division, x - c s, is exact in one fma (the tie goes to the even code).
 __device__ __forceinline__ float code_of(float x, float s, float rs) {
   const float c = rintf(x * rs), rest = fmaf(-c, s, x), h = 0.5f * s;
   const float up = rest < 0.f ? -1.f : 1.f, far = fabsf(rest);
   const bool odd = ((int)c & 1) != 0;
   return far > h || (far == h && odd) ? c + up : c;
 }
-__device__ __forceinline__ float code_guess(float x, float rs, bool &near) {
-  const float y = x * rs, c = rintf(y);
-  near |= !(fabsf(y - c) <= 0.5f - 0x1p-15f);
-  return c;
+// A float whose low byte is x rs rounded (at 1.5 * 2^23 a step is 1); `far`: the
+// largest distance from it so far.
+__device__ __forceinline__ uint32_t code_guess(float x, float rs, float &far) {
+  const float y = fmaf(x, rs, 0x1.8p23f);
+  far = fmaxf(far, fabsf(fmaf(x, rs, -(y - 0x1.8p23f))));
+  return __float_as_uint(y);
+}
+constexpr float CODE_SURE = 0.5f - 0x1p-15f;
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t *y) {
+  return __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u) | __builtin_amdgcn_perm(y[3], y[2], 0x04000c0cu);
+}
+
+// The largest magnitude of vectors of T as whole numbers, which order as the
+// values do, infinities and NaN last; 16-bit types in pairs.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+template <class T>
+__device__ __forceinline__ void largest_of(uint32_t w, uint32_t &top) {
+  if (sizeof(T) == 4)
+    top = max(top, w & 0x7fffffffu);
+  else
+    top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+// Its value; infinity where it is not finite.
+template <class T>
+__device__ __forceinline__ float largest_value(uint32_t top) {
+  float f = __uint_as_float(top);
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t t = (uint16_t)max(top & 0xffffu, top >> 16);
+    f = to_f32(__builtin_bit_cast(T, t));
+  }
+  return f <= 3.4028234663852886e38f ? f : __builtin_inff();
 }
 
 // One run of `len` rows from token t on, by W waves; `top` and `bad` of each
@@ -300,22 +326,18 @@ __device__ __forceinline__ void append_run(const AppendArgs &a, int t, int slot,
 #pragma unroll
   for (int i = 0; i < KEEP; i++)
     if (row + i * RPI < len) kept[i] = *(const V *)(src + (row + i * RPI) * stride + d);
-  float top = 0.f;
-  bool bad = false;
+  uint32_t bits = 0;
   auto look = [&](const V &x) {
+    uint32_t w[4];
+    __builtin_memcpy(w, &x, 16);
 #pragma unroll
-    for (int e = 0; e < VE; e++) {
-      const float f = fabsf(to_f32(x.v[e]));
-      bad |= !(f <= 3.4028234663852886e38f);
-      top = fmaxf(top, f);
-    }
+    for (int e = 0; e < 4; e++) largest_of<T>(w[e], bits);
   };
 #pragma unroll
   for (int i = 0; i < KEEP; i++)
     if (row + i * RPI < len) look(kept[i]);
   for (int r = row + KEEP * RPI; r < len; r += RPI) look(*(const V *)(src + r * stride + d));
-  top = wave_max(top);
-  if (__any(bad)) top = __builtin_inff();
+  float top = wave_max(largest_value<T>(bits));
   if (W > 1) {
     if ((me & 63) == 0) tops[me / 64] = top;
     __syncthreads();
@@ -326,15 +348,15 @@ __device__ __forceinline__ void append_run(const AppendArgs &a, int t, int slot,
   const float now = top == __builtin_inff() || old != old ? __builtin_nanf("") : fmaxf(fmaxf(old, top / 127.0f), KV8_MIN_SCALE);
   if (now > old && old > 0.f) {
     const double s0 = old, s1 = now;
-    const float ratio = (float)(s0 / s1);  // (as above: |c| ratio is off by less than 2^-15 / 2)
+    const float ratio = (float)(s0 / s1);  // (as above: c ratio is off by less than 128 * 2^-24)
     for (int i = 4 * me; i < off * HD; i += W * 256) {
       const uint32_t w = *(const uint32_t *)(codes + i);
-      uint32_t y = 0;
-      bool near = false;
+      uint32_t c[4], y;
+      float far = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        y |= ((uint32_t)(int)code_guess((float)(int8_t)(w >> (8 * e)), ratio, near) & 0xffu) << (8 * e);
-      if (near) {
+      for (int e = 0; e < 4; e++) c[e] = code_guess((float)(int8_t)(w >> (8 * e)), ratio, far);
+      y = low_bytes(c);
+      if (far > CODE_SURE) {
         y = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -345,11 +367,13 @@ __device__ __forceinline__ void append_run(const AppendArgs &a, int t, int slot,
   }
   const float rs = 1.0f / now;
   auto put = [&](const V &x, int r) {
-    uint32_t w[VE / 4] = {};
-    bool near = false;
+    uint32_t w[VE / 4], c[VE];
+    float far = 0.f;
 #pragma unroll
-    for (int e = 0; e < VE; e++) w[e / 4] |= ((uint32_t)(int)code_guess(to_f32(x.v[e]), rs, near) & 0xffu) << (8 * (e & 3));
-    if (near) {  // (a NaN scale too: its codes are zeros)
+    for (int e = 0; e < VE; e++) c[e] = code_guess(to_f32(x.v[e]), rs, far);
+#pragma unroll
+    for (int k = 0; k < VE / 4; k++) w[k] = low_bytes(c + 4 * k);
+    if (far > CODE_SURE || now != now) {  // (a NaN scale: zeros)
 #pragma unroll
       for (int k = 0; k < VE / 4; k++) w[k] = 0;
 #pragma unroll
@@ -381,23 +405,35 @@ __global__ __launch_bounds__(APPEND_THREADS) void k_kv8_append(AppendArgs a) {
   const int w0 = ((wb | 31) < (int)(gridDim.x / a.heads) ? turned : wb) * a.window;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const bool isv = blockIdx.y;
-  // the window's tokens, one a lane: those that begin a run, those that go on
-  const int t = w0 + lane, wide = min(a.window, a.n - w0);
-  const int slot = lane < wide ? a.slots[t] : -1;
-  const int before = lane < wide && t ? a.slots[t - 1] : -1;
-  const bool fits = slot >= 0 && slot < a.total;
-  const bool goes_on = fits && slot % a.page && before == slot - 1;
-  const unsigned long long begins = __ballot(fits && !goes_on), other = __ballot(lane < wide && !goes_on);
+  // The window's tokens and those behind it, two a lane: which begin a run, which
+  // go on (128 at once: the end of a run of 64 waits for no further read).
+  const int wide = min(a.window, a.n - w0);
+  int slot[2], before[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const int t = w0 + 64 * k + lane;
+    slot[k] = t < a.n ? a.slots[t] : -1;
+    before[k] = t < a.n && t ? a.slots[t - 1] : -1;
+  }
+  unsigned long long stops[2], begins = 0;
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const bool fits = slot[k] >= 0 && slot[k] < a.total, goes_on = fits && slot[k] % a.page && before[k] == slot[k] - 1;
+    stops[k] = __ballot(!goes_on);
+    if (k == 0) begins = __ballot(lane < wide && fits && !goes_on);
+  }
   int short_run = 0, long_run = 0;
   for (unsigned long long left = begins; left; left &= left - 1) {
-    const int i = __ffsll(left) - 1, first = __shfl(slot, i);
-    const unsigned long long next = i < 63 ? other >> (i + 1) : 0;
+    const int i = __ffsll(left) - 1, first = __shfl(slot[0], i);
+    const unsigned long long next = i < 63 ? stops[0] >> (i + 1) : 0;
     int len;
     if (next) {
       len = __ffsll(next);
-    } else {  // to the window's end, then on in steps of 64
+    } else if (stops[1]) {
+      len = 63 - i + __ffsll(stops[1]);
+    } else {  // on in steps of 64
       const int most = min(a.page - first % a.page, a.n - (w0 + i));
-      len = wide - i;
+      len = 128 - i;
       while (len < most) {
         const int j = len + lane;
         const unsigned long long no = __ballot(j >= most || a.slots[w0 + i + j] != first + j);

@@ -344,9 +344,9 @@ int gq_rope(int dtype, int layout, int n, int head_dim, int rot_dim, const doubl
  * with the quotients exact and ties to even.  Rows behind them keep their codes.
  * A value that is not finite makes the scale NaN until rows start the page
  * anew; requests that do not see the page are not touched by it.
- * The rows that a call writes into a page are neighbours in the call, in the
- * order of their slots (gq_page_plan's are); what a page holds after a call
- * that breaks this is not specified.  Buffers and strides are multiples of 16
+ * The rows that a call writes into a page follow each other in the call and in
+ * the page, at slots s, s + 1, ... (gq_page_plan's do); what a page holds after
+ * a call that breaks this is not specified.  Buffers and strides are multiples of 16
  * bytes; n * n_kv_heads < 2^28. */
 int gq_kv8_append(const gq_kv8 *cache, int dtype, const void *k_dev, int64_t k_stride, const void *v_dev,
                   int64_t v_stride, const int *slots_dev, int n, void *stream);
