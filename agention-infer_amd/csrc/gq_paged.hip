@@ -260,8 +260,9 @@ hipError_t launch_rope(const RopeArgs &a, int dtype, hipStream_t st) {
 // beginnings in a window of tokens (at one head of k or v): a run of up to
 // APPEND_SHORT rows is one wave's, a longer one the whole block's.  Rows stay in
 // registers between the maximum and the codes.  64 single tokens of 4 heads in
-// 4.4 us; 8184 tokens of 24 prompts, 8 bf16 heads, in 23 us (2.2 TB/s: the
-// reads of slots, rows and scales wait for one another).
+// 4.4 us; 8184 tokens of 24 prompts, 8 bf16 heads, in 21.6 us (2.3 TB/s: the
+// reads of slots, rows and scales wait for one another); 65536 of 8 f32 heads at
+// 4.3 TB/s.
 constexpr int APPEND_THREADS = 256, APPEND_WAVES = APPEND_THREADS / 64, APPEND_SHORT = 16;
 
 // rint(x / s) for finite x, |x| <= 127.5 s, rs = 1 / s (s >= 2^-60).  x rs is off
@@ -394,7 +395,7 @@ __device__ __forceinline__ void append_run(const AppendArgs &a, int t, int slot,
 }
 
 template <class T, int HD>
-__global__ __launch_bounds__(APPEND_THREADS) void k_kv8_append(AppendArgs a) {
+__global__ __launch_bounds__(APPEND_THREADS, 4) void k_kv8_append(AppendArgs a) {
   __shared__ float tops[2][APPEND_WAVES];
   // Heads go fastest: blocks that run together read whole rows.  Runs of whole
   // pages begin in every second, fourth, ... window, and blocks go to the CUs
@@ -457,8 +458,9 @@ static void append_launch(AppendArgs a, int hd, hipStream_t st) {
   // another.  Calls of single tokens x heads in windows of 4 / 16 / 32, bf16:
   // 256 x 8 15.0 / 19.8 / 27.4 us, 1024 x 8 27.9 / 23.2 / 28.9, 4096 x 8 72 /
   // 54.7 / 53.6; prompts 512 x 4 17.8 / 17.5 / 17.8, 8192 x 8 55 / 39.3 / 36.6.
+  // Prompts in windows of 32 / 64: 8192 x 8 35.5 / 36.8, 65536 x 8 169 / 153.
   const int64_t rows = (int64_t)a.n * a.heads;
-  a.window = rows <= 4096 ? APPEND_WAVES : rows < 32768 ? 16 : 32;
+  a.window = rows <= 4096 ? APPEND_WAVES : rows < 32768 ? 16 : rows < 131072 ? 32 : 64;
   const dim3 g((unsigned)(((int64_t)a.n + a.window - 1) / a.window * a.heads), 2), b(APPEND_THREADS);
   if (hd == 64)
     hipLaunchKernelGGL((k_kv8_append<T, 64>), g, b, 0, st, a);

@@ -321,7 +321,8 @@ def test_append_and_read(backend, dtype, page, heads, hd):
     (3, 64, 16, [1] * 900 + [5] * 90),              # single tokens, drafts
     (8, 128, 64, [700, 1, 64, 1, 2, 129, 300, 17] + [1] * 40),
     (8, 64, 256, [1500, 255, 257, 1, 2000, 31, 33]),
-    (16, 64, 48, [1, 2, 3, 16, 17, 18, 47, 48, 49] * 11)])
+    (16, 64, 48, [1, 2, 3, 16, 17, 18, 47, 48, 49] * 11),
+    (32, 64, 64, [1] * 70 + [1000, 15, 64, 333, 2, 129, 2000, 63, 65, 700])])
 def test_append_many(backend, dtype, heads, hd, page, lengths):
     """Passes of hundreds and thousands of rows: runs of every length that
     begin anywhere, twice, the second time behind the first."""
